@@ -183,6 +183,57 @@ int pk_decode_set_fast_path(int warps);
 void pk_decode_set_spin_limit(unsigned rounds);
 int pk_decode_wait_probe(void* workspace, size_t bytes, unsigned rounds, void* stream);
 
+/* ---------------------------------------------------------------- paged KV cache in 8 bits, attention over it */
+
+/* No counterpart in the reference (its caches are bf16).  Values e4m3, one E8M0 scale per (page, kv head) for K and one
+ * for V (x = value * 2^(scale - 127)); head_dim is 64.  K and V of (page, head, slot) are 64 bytes at
+ * page * page_stride + head * head_stride + slot * token_stride + k_off / v_off; all strides and offsets are bytes and
+ * multiples of 16, page_size is 16, 32, 64, 128 or 256.  block_table int32 [batch][bt_cols] (row stride bt_stride
+ * elements); an entry outside 0..pages-1 stands for no page: nothing is stored there and its tokens are masked.
+ * seq_lens int32 [batch] include the new tokens.  cu_seqlens int32 [batch + 1]: request r owns rows
+ * cu[r]..cu[r+1]-1 of q / k / v, the last cu[r+1]-cu[r] positions of its sequence; NULL: row r is request r. */
+typedef struct PkKv8Cache {
+    void* cache; void* scales;              /* scales uint8 [pages][kv_heads][2] (K, V), contiguous */
+    long long k_off, v_off, page_stride, token_stride, head_stride;
+    int pages, page_size, kv_heads;
+    const void* block_table; long long bt_stride; int bt_cols;
+    const void* seq_lens; const void* cu_seqlens; int batch;
+} PkKv8Cache;
+
+/* Store bf16 K and V rows [tokens, kv_heads, 64] (strides in elements, multiples of 8).  A page whose slot 0 is among the
+ * new tokens takes the scale 2^ceil(log2(amax / 448)) of its new tokens; a page begun earlier takes the larger of that
+ * and its own, and tokens already held are re-rounded when the scale grows.  NaN and Inf do not count for amax; Inf
+ * saturates.  A page that is written to belongs to one request only. */
+int pk_kv8_append(const PkKv8Cache* cache, const void* k, long long k_token_stride, long long k_head_stride, const void* v,
+                  long long v_token_stride, long long v_head_stride, int tokens, void* stream);
+/* Causal attention of bf16 q rows [tokens, q_heads, 64] over the cache, q_heads a multiple of kv_heads; out bf16 of the
+ * same shape, lse fp32 [tokens][q_heads] (nullable, natural log).  A row that sees no key gets 0 and -inf; rows of no
+ * request are left as they are.  max_query_len: the longest cu[r+1]-cu[r] (0: unknown; a smaller one costs time only). */
+int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long long q_token_stride, long long q_head_stride, void* out,
+                     long long out_token_stride, long long out_head_stride, void* lse, int tokens, int q_heads,
+                     int max_query_len, float scale, void* stream);
+
+/* ---------------------------------------------------------------- sampling */
+
+/* Draw one token per row of logits [rows, vocab] (dtype 0 bf16, 1 fp16, 2 fp32; row_stride in elements; vocab <= 262144)
+ * from the given uniform numbers (fp32 [rows], 0 <= u < 1).  No counterpart in the reference (its decode ends before the
+ * lm_head).  w_i = exp((l_i - max) / temperature), tokens ordered by logit (ties: lower index first); the first top_k
+ * stay, of those the shortest prefix that holds top_p of their weight, of those the ones with w_i >= min_p; the token
+ * drawn is the lowest index at which the running sum of kept weights, in index order, exceeds u times their sum.  The
+ * most likely token always stays.  temperature <= 0 or NaN: the largest logit, lowest index.  top_k <= 0, top_p >= 1 and
+ * min_p <= 0 are off.  NaN and -inf are never drawn; a row of nothing else gives id 0 and logprob NaN.
+ * Each setting is a device array [rows] (top_k int32, others fp32) or, where that is NULL, its _value.
+ * ids int64 [rows]; logprobs fp32 [rows] (nullable): log of the drawn token's share of the kept weight, 0 when greedy. */
+typedef struct PkSampleArgs {
+    void* stream;
+    const void* logits; long long row_stride; int rows, vocab, dtype;
+    const void* uniform;
+    const void *temperature, *top_k, *top_p, *min_p;
+    float temperature_value; int top_k_value; float top_p_value, min_p_value;
+    void* ids; void* logprobs;
+} PkSampleArgs;
+int pk_sample(const PkSampleArgs* args);
+
 /* ---------------------------------------------------------------- drop-in signatures of the reference */
 
 /* SmolLM2-135M: prime_kernels/decode_megakernel/csrc/megakernel.cu:833-927 (same arguments, same

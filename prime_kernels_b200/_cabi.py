@@ -35,6 +35,19 @@ class PkDecodeArgs(ctypes.Structure):
                 ("lm_head", ci), ("advance", ci)]
 
 
+class PkKv8Cache(ctypes.Structure):
+    _fields_ = [("cache", vp), ("scales", vp), ("k_off", ll), ("v_off", ll), ("page_stride", ll), ("token_stride", ll),
+                ("head_stride", ll), ("pages", ci), ("page_size", ci), ("kv_heads", ci), ("block_table", vp),
+                ("bt_stride", ll), ("bt_cols", ci), ("seq_lens", vp), ("cu_seqlens", vp), ("batch", ci)]
+
+
+class PkSampleArgs(ctypes.Structure):
+    _fields_ = [("stream", vp), ("logits", vp), ("row_stride", ll), ("rows", ci), ("vocab", ci), ("dtype", ci),
+                ("uniform", vp), ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp),
+                ("temperature_value", cf), ("top_k_value", ci), ("top_p_value", cf), ("min_p_value", cf), ("ids", vp),
+                ("logprobs", vp)]
+
+
 # name -> (restype, argtypes): every symbol include/prime_kernels_b200.h declares
 SYMBOLS = {
     "pk_fused_rmsnorm_residual_forward": (ci, [vp, vp, vp, vp, vp, vp, cf, ci, ci, vp]),
@@ -69,6 +82,9 @@ SYMBOLS = {
     "pk_decode_set_fast_path": (ci, [ci]),
     "pk_decode_set_spin_limit": (None, [ctypes.c_uint]),
     "pk_decode_wait_probe": (ci, [vp, sz, ctypes.c_uint, vp]),
+    "pk_kv8_append": (ci, [ctypes.POINTER(PkKv8Cache), vp, ll, ll, vp, ll, ll, ci, vp]),
+    "pk_kv8_attention": (ci, [ctypes.POINTER(PkKv8Cache), vp, ll, ll, vp, ll, ll, vp, ci, ci, ci, cf, vp]),
+    "pk_sample": (ci, [ctypes.POINTER(PkSampleArgs)]),
     "mk_query": (ci, [ip] * 7),
     "mk_workspace_bytes": (sz, [ci, ci]),
     "mk_decode": (ci, [vp, ci, vp, ci, vp, vp, vp, ci, vp, vp, vp, vp, vp, ll, ll, ll, ll, ll, ci, vp, ci, vp, vp, sz, ci]),

@@ -258,7 +258,193 @@ std::tuple<torch::Tensor, torch::Tensor> swiglu_bwd(const torch::Tensor& grad, c
     return {d_gate, d_up};
 }
 
+// ---- paged KV cache in 8 bits
+// The cache is [pages, kv_heads, page_size, 128] (K in 0..63, V in 64..127) or [2, pages, page_size, kv_heads, 64].
+PkKv8Cache kv8_cache(const torch::Tensor& cache, const torch::Tensor& scales, const torch::Tensor& block_table,
+                     const torch::Tensor& seq_lens, const std::optional<torch::Tensor>& cu_seqlens, int64_t tokens) {
+    TORCH_CHECK(cache.is_cuda() && (cache.dtype() == torch::kFloat8_e4m3fn || cache.dtype() == torch::kUInt8),
+                "cache must be a CUDA float8_e4m3fn (or uint8) tensor");
+    TORCH_CHECK(scales.dtype() == torch::kFloat8_e8m0fnu || scales.dtype() == torch::kUInt8,
+                "scales must be a float8_e8m0fnu (or uint8) tensor");
+    PkKv8Cache c{};
+    if (cache.dim() == 4) {
+        TORCH_CHECK(cache.size(3) == 128 && cache.stride(3) == 1, "a 4-D cache must be [pages, kv_heads, page_size, 128] with unit last stride");
+        c.pages = (int)cache.size(0); c.kv_heads = (int)cache.size(1); c.page_size = (int)cache.size(2);
+        c.v_off = 64;
+        c.page_stride = cache.stride(0); c.head_stride = cache.stride(1); c.token_stride = cache.stride(2);
+    } else {
+        TORCH_CHECK(cache.dim() == 5 && cache.size(0) == 2 && cache.size(4) == 64 && cache.stride(4) == 1,
+                    "cache must be [pages, kv_heads, page_size, 128] or [2, pages, page_size, kv_heads, 64] with unit last stride");
+        c.pages = (int)cache.size(1); c.page_size = (int)cache.size(2); c.kv_heads = (int)cache.size(3);
+        c.v_off = cache.stride(0);
+        c.page_stride = cache.stride(1); c.token_stride = cache.stride(2); c.head_stride = cache.stride(3);
+    }
+    TORCH_CHECK(c.page_size == 16 || c.page_size == 32 || c.page_size == 64 || c.page_size == 128 || c.page_size == 256,
+                "page_size must be 16, 32, 64, 128 or 256, got ", c.page_size);
+    TORCH_CHECK(cache.size(cache.dim() == 4 ? 0 : 1) <= INT32_MAX, "too many pages");
+    TORCH_CHECK(scales.dim() == 3 && scales.size(0) == c.pages && scales.size(1) == c.kv_heads && scales.size(2) == 2 && scales.is_contiguous(),
+                "scales must be contiguous [pages, kv_heads, 2]");
+    TORCH_CHECK(block_table.dim() == 2 && block_table.dtype() == torch::kInt32 && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+                "block_table must be int32 [batch, columns] with contiguous rows");
+    TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.dtype() == torch::kInt32 && seq_lens.is_contiguous(), "seq_lens must be contiguous int32 [batch]");
+    const int64_t batch = seq_lens.size(0);
+    TORCH_CHECK(block_table.size(0) >= batch, "block_table must have a row for each request");
+    TORCH_CHECK(tokens <= INT32_MAX && block_table.size(1) * c.page_size <= INT32_MAX, "sizes must fit 32 bits");
+    if (cu_seqlens.has_value()) {
+        TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->dtype() == torch::kInt32 && cu_seqlens->is_contiguous() &&
+                        cu_seqlens->size(0) == batch + 1, "cu_seqlens must be contiguous int32 [batch + 1]");
+        TORCH_CHECK(cu_seqlens->device() == cache.device(), "all inputs must be on the same device");
+        c.cu_seqlens = cu_seqlens->const_data_ptr();
+    } else {
+        TORCH_CHECK(tokens >= batch, "without cu_seqlens every request needs a row");
+    }
+    TORCH_CHECK(scales.device() == cache.device() && block_table.device() == cache.device() && seq_lens.device() == cache.device(),
+                "all inputs must be on the same device");
+    c.cache = const_cast<void*>(cache.const_data_ptr());
+    c.scales = const_cast<void*>(scales.const_data_ptr());
+    c.block_table = block_table.const_data_ptr();
+    c.bt_stride = block_table.stride(0);
+    c.bt_cols = (int)block_table.size(1);
+    c.seq_lens = seq_lens.const_data_ptr();
+    c.batch = (int)batch;
+    return c;
+}
+
+void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& cache) {
+    TORCH_CHECK(t.dtype() == torch::kBFloat16 && t.dim() == 3 && t.size(2) == 64 && t.stride(2) == 1, name,
+                " must be bfloat16 [tokens, heads, 64] with unit last stride");
+    TORCH_CHECK(t.device() == cache.device(), "all inputs must be on the same device");
+    TORCH_CHECK(t.numel() == 0 || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0),
+                name, " must be 16-byte aligned with strides that are multiples of 8 elements");
+}
+
+void kv8_append(const torch::Tensor& k, const torch::Tensor& v, torch::Tensor cache, torch::Tensor scales,
+                const torch::Tensor& block_table, const torch::Tensor& seq_lens, const std::optional<torch::Tensor>& cu_seqlens) {
+    TORCH_CHECK(k.dim() == 3, "k must be bfloat16 [tokens, heads, 64] with unit last stride");
+    const PkKv8Cache c = kv8_cache(cache, scales, block_table, seq_lens, cu_seqlens, k.size(0));
+    check_rows(k, "k", cache);
+    check_rows(v, "v", cache);
+    TORCH_CHECK(k.size(1) == c.kv_heads && v.sizes() == k.sizes(), "k and v must be [tokens, kv_heads, 64]");
+    at::cuda::OptionalCUDAGuard guard{device_of(cache)};
+    const int rc = pk_kv8_append(&c, k.const_data_ptr(), k.stride(0), k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1),
+                                 (int)k.size(0), at::cuda::getCurrentCUDAStream());
+    TORCH_CHECK(rc == 0, "kv8 append failed: ", pk_status_string(rc));
+}
+
+void kv8_attention_out(const torch::Tensor& q, const torch::Tensor& cache, const torch::Tensor& scales,
+                       const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                       const std::optional<torch::Tensor>& cu_seqlens, int64_t max_query_len, double scale, torch::Tensor out,
+                       std::optional<torch::Tensor> lse) {
+    TORCH_CHECK(q.dim() == 3, "q must be bfloat16 [tokens, heads, 64] with unit last stride");
+    const PkKv8Cache c = kv8_cache(cache, scales, block_table, seq_lens, cu_seqlens, q.size(0));
+    check_rows(q, "q", cache);
+    check_rows(out, "out", cache);
+    TORCH_CHECK(c.kv_heads > 0 && q.size(1) > 0 && q.size(1) % c.kv_heads == 0, "q heads must be a multiple of kv heads");
+    TORCH_CHECK(out.sizes() == q.sizes(), "out must have the shape of q");
+    TORCH_CHECK(max_query_len >= 0 && max_query_len <= INT32_MAX, "max_query_len must be 0 (unknown) or positive");
+    if (lse.has_value())
+        TORCH_CHECK(lse->dtype() == torch::kFloat32 && lse->dim() == 2 && lse->size(0) == q.size(0) && lse->size(1) == q.size(1) &&
+                        lse->is_contiguous() && lse->device() == cache.device(), "lse must be contiguous float32 [tokens, heads]");
+    at::cuda::OptionalCUDAGuard guard{device_of(cache)};
+    const int rc = pk_kv8_attention(&c, q.const_data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                    opt_mptr(lse), (int)q.size(0), (int)q.size(1), (int)max_query_len, (float)scale,
+                                    at::cuda::getCurrentCUDAStream());
+    TORCH_CHECK(rc == 0, "kv8 attention failed: ", pk_status_string(rc));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv8_attention(const torch::Tensor& q, const torch::Tensor& cache,
+                                                       const torch::Tensor& scales, const torch::Tensor& block_table,
+                                                       const torch::Tensor& seq_lens, const std::optional<torch::Tensor>& cu_seqlens,
+                                                       int64_t max_query_len, double scale, bool return_lse) {
+    torch::Tensor out = torch::empty(q.sizes(), q.options());
+    torch::Tensor lse = return_lse && q.dim() == 3 ? torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32))
+                                                   : torch::empty({0}, q.options().dtype(torch::kFloat32));
+    kv8_attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, out,
+                      return_lse ? std::optional<torch::Tensor>(lse) : std::nullopt);
+    return {out, lse};
+}
+
+// ---- sampling
+void sample_out(const torch::Tensor& logits, const torch::Tensor& uniform, const std::optional<torch::Tensor>& temperature,
+                double temperature_value, const std::optional<torch::Tensor>& top_k, int64_t top_k_value,
+                const std::optional<torch::Tensor>& top_p, double top_p_value, const std::optional<torch::Tensor>& min_p,
+                double min_p_value, torch::Tensor ids, std::optional<torch::Tensor> logprobs) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
+    TORCH_CHECK(logits.dtype() == torch::kBFloat16 || logits.dtype() == torch::kHalf || logits.dtype() == torch::kFloat32,
+                "logits must be bfloat16, float16 or float32");
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK(vocab > 0 && vocab <= 262144 && (vocab == 1 || logits.stride(1) == 1), "vocab must be 1..262144 with unit stride");
+    TORCH_CHECK(rows <= (1 << 24), "too many rows");
+    auto per_row = [&](const torch::Tensor& t, const char* name, torch::ScalarType type) {
+        TORCH_CHECK(t.dtype() == type && t.dim() == 1 && t.size(0) == rows && t.is_contiguous() && t.device() == logits.device(),
+                    name, " must be contiguous ", type, " [rows] on the device of the logits");
+    };
+    per_row(uniform, "uniform", torch::kFloat32);
+    if (temperature.has_value()) per_row(*temperature, "temperature", torch::kFloat32);
+    if (top_k.has_value()) per_row(*top_k, "top_k", torch::kInt32);
+    if (top_p.has_value()) per_row(*top_p, "top_p", torch::kFloat32);
+    if (min_p.has_value()) per_row(*min_p, "min_p", torch::kFloat32);
+    per_row(ids, "ids", torch::kInt64);
+    if (logprobs.has_value()) per_row(*logprobs, "logprobs", torch::kFloat32);
+    PkSampleArgs a{};
+    at::cuda::OptionalCUDAGuard guard{device_of(logits)};
+    a.stream = at::cuda::getCurrentCUDAStream();
+    a.logits = logits.const_data_ptr();
+    a.row_stride = logits.stride(0);
+    a.rows = (int)rows;
+    a.vocab = (int)vocab;
+    a.dtype = logits.dtype() == torch::kBFloat16 ? 0 : (logits.dtype() == torch::kHalf ? 1 : 2);
+    a.uniform = uniform.const_data_ptr();
+    a.temperature = opt_ptr(temperature);
+    a.top_k = opt_ptr(top_k);
+    a.top_p = opt_ptr(top_p);
+    a.min_p = opt_ptr(min_p);
+    a.temperature_value = (float)temperature_value;
+    a.top_k_value = (int)std::min<int64_t>(top_k_value, INT32_MAX);
+    a.top_p_value = (float)top_p_value;
+    a.min_p_value = (float)min_p_value;
+    a.ids = ids.data_ptr();
+    a.logprobs = opt_mptr(logprobs);
+    const int rc = pk_sample(&a);
+    TORCH_CHECK(rc == 0, "sample failed: ", pk_status_string(rc));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, const torch::Tensor& uniform,
+                                                const std::optional<torch::Tensor>& temperature, double temperature_value,
+                                                const std::optional<torch::Tensor>& top_k, int64_t top_k_value,
+                                                const std::optional<torch::Tensor>& top_p, double top_p_value,
+                                                const std::optional<torch::Tensor>& min_p, double min_p_value, bool return_logprobs) {
+    TORCH_CHECK(logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
+    auto opts = torch::TensorOptions().device(logits.device());
+    torch::Tensor ids = torch::empty({logits.size(0)}, opts.dtype(torch::kInt64));
+    torch::Tensor lp = torch::empty({return_logprobs ? logits.size(0) : 0}, opts.dtype(torch::kFloat32));
+    sample_out(logits, uniform, temperature, temperature_value, top_k, top_k_value, top_p, top_p_value, min_p, min_p_value, ids,
+               return_logprobs ? std::optional<torch::Tensor>(lp) : std::nullopt);
+    return {ids, lp};
+}
+
 }  // namespace
+
+TORCH_LIBRARY_FRAGMENT(prime_kv8, m) {
+    m.def("append(Tensor k, Tensor v, Tensor(a!) cache, Tensor(b!) scales, Tensor block_table, Tensor seq_lens, "
+          "Tensor? cu_seqlens) -> ()");
+    m.impl("append", torch::kCUDA, &kv8_append);
+    m.def("attention(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
+          "int max_query_len, float scale, bool return_lse) -> (Tensor, Tensor)");
+    m.impl("attention", torch::kCUDA, &kv8_attention);
+    m.def("attention_out(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
+          "int max_query_len, float scale, Tensor(a!) out, Tensor(b!)? lse) -> ()");
+    m.impl("attention_out", torch::kCUDA, &kv8_attention_out);
+}
+
+TORCH_LIBRARY_FRAGMENT(prime_sampling, m) {
+    m.def("sample(Tensor logits, Tensor uniform, Tensor? temperature, float temperature_value, Tensor? top_k, int top_k_value, "
+          "Tensor? top_p, float top_p_value, Tensor? min_p, float min_p_value, bool return_logprobs) -> (Tensor, Tensor)");
+    m.impl("sample", torch::kCUDA, &sample);
+    m.def("sample_out(Tensor logits, Tensor uniform, Tensor? temperature, float temperature_value, Tensor? top_k, int top_k_value, "
+          "Tensor? top_p, float top_p_value, Tensor? min_p, float min_p_value, Tensor(a!) ids, Tensor(b!)? logprobs) -> ()");
+    m.impl("sample_out", torch::kCUDA, &sample_out);
+}
 
 TORCH_LIBRARY_FRAGMENT(prime_elementwise, m) {
     m.def("apply_rotary(Tensor q, Tensor k, Tensor cos, Tensor sin, int unsqueeze_dim) -> (Tensor, Tensor)");

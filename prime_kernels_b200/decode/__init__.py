@@ -331,8 +331,9 @@ def check_status(geometry: Geometry, device) -> None:
 
 
 class DecodeSession:
-    """Greedy generation driver: all step inputs live on the device and the kernel advances them in
-    place (``advance=True``), so ``steps`` launches run back to back with no host round trip."""
+    """Generation driver: all step inputs live on the device and the kernel advances them in place
+    (``advance=True``), so ``steps`` launches run back to back with no host round trip.  Greedy, or with a
+    :class:`prime_kernels_b200.sampling.Sampler` drawing each next id from the step's logits."""
 
     def __init__(self, geometry: Geometry, *, embed, layers, final_norm, kv_caches, cos_sin_cache, block_table,
                  embed_lookup=None):
@@ -354,20 +355,25 @@ class DecodeSession:
         blk = bt[rows, (self.positions // self.block_size).long()].to(torch.int64)
         self.slot_mapping = blk * self.block_size + self.positions % self.block_size
 
-    def step(self):
-        return decode_step(self.geometry, input_ids=self.input_ids, positions=self.positions,
-                           seq_lens=self.seq_lens, block_table=self.block_table, slot_mapping=self.slot_mapping,
-                           embed=self.embed, layers=self.layers, final_norm=self.final_norm,
-                           kv_caches=self.kv_caches, cos_sin_cache=self.cos_sin_cache, eps=self.geometry.eps,
-                           lm_head=True, advance=True, embed_lookup=self.embed_lookup)
+    def step(self, sampler=None):
+        hidden, logits, next_ids = decode_step(
+            self.geometry, input_ids=self.input_ids, positions=self.positions,
+            seq_lens=self.seq_lens, block_table=self.block_table, slot_mapping=self.slot_mapping,
+            embed=self.embed, layers=self.layers, final_norm=self.final_norm,
+            kv_caches=self.kv_caches, cos_sin_cache=self.cos_sin_cache, eps=self.geometry.eps,
+            lm_head=True, advance=True, embed_lookup=self.embed_lookup)
+        if sampler is not None:
+            # the kernel has advanced the step inputs with the greedy ids: the drawn ones take their place
+            self.input_ids.copy_(sampler(logits, out=next_ids))
+        return hidden, logits, next_ids
 
-    def generate(self, steps: int, collect_logits: bool = False):
-        """Run ``steps`` greedy steps; returns ids ``[steps, B]`` (and logits ``[steps, B, V]``)."""
+    def generate(self, steps: int, collect_logits: bool = False, sampler=None):
+        """Run ``steps`` steps, greedy or drawing with ``sampler``; returns ids ``[steps, B]`` (and logits ``[steps, B, V]``)."""
         b = self.input_ids.shape[0]
         ids = torch.empty((steps, b), dtype=torch.int64, device=self.device)
         logs = torch.empty((steps, b, self.geometry.vocab), dtype=torch.bfloat16, device=self.device) if collect_logits else None
         for t in range(steps):
-            _, logits, next_ids = self.step()
+            _, logits, next_ids = self.step(sampler)
             ids[t].copy_(next_ids)
             if collect_logits:
                 logs[t].copy_(logits)
