@@ -45,10 +45,10 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {     // low 16 bits; exact
-    uint32_t r;
-    asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
-    return r;
+// four e4m3 values to two f16x2 words; exact
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi) : "r"(four));
 }
 
 // request of token t (last r with cu[r] <= t) and its token range, clamped to the rows there are; false: no request
@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(AppendParams p) {
                     uint32_t* w = reinterpret_cast<uint32_t*>(&a);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t lo = e4m3x2_to_f16x2(w[j] & 0xffffu), hi = e4m3x2_to_f16x2(w[j] >> 16);
+                        uint32_t lo, hi;
+                        e4m3x4_to_f16(w[j], lo, hi);
                         const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&lo));
                         const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                         w[j] = e4m3x2(fl.x * f, fl.y * f) | (e4m3x2(fh.x * f, fh.y * f) << 16);
@@ -155,17 +156,24 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(AppendParams p) {
 }
 
 // ---------------------------------------------------------------- attention
-// Rows of one (request, kv head): (token, query head of the group), row = token * G + head; tiles of 16 rows.  A
-// tile's keys are dealt to the CTAs of a cluster and, in steps of 16 keys, to the warps of a CTA; every warp keeps a
+// Rows of one (request, kv head): (token, query head of the group), row = token * G + head; tiles of 8 or 16 rows.  A
+// tile's keys are dealt to the CTAs of a cluster and, in steps of 32 keys, to the warps of a CTA; every warp keeps a
 // running softmax of its own (one pass over the cache), merged at the end in shared memory and then through
 // distributed shared memory.  Products run on m16n8k16 f16 with fp32 accumulation: e4m3 converts to f16 exactly, and
 // q is divided by a power of two per row so that its bf16 bits fit f16 (elements 2^-22 below the row's largest lose
-// bits).  The cache goes from global memory straight into the operand registers: a lane's 16 bytes of a K row are
-// its dims of all four k-steps, and pairs of V rows are interleaved by byte permutation.
+// bits).  The cache reaches the operand registers by way of a ring of its own for every warp (asynchronous 16-byte
+// copies, no barrier but the warp's): a lane's 16 bytes of a K row are its dims of all four k-steps, and pairs of V rows
+// are interleaved by byte permutation.
 //
 // V scales differ from page to page, so weights enter the second product as 2^(s + eV - top) with a running maximum
 // `top` of s + eV of their own, apart from the running maximum of s that the sum uses: neither over- nor underflows
 // whatever the scales are.
+//
+// Bound by the bytes of the cache where there are many, by the chain of dependent reads at the start (length, page, page's
+// data) and the merge where there are few.  64 requests of up to 8192 tokens, 15/5 heads: 44 us, 4.8 TB/s, 0.73 of the
+// measured copy bandwidth.  Steps of 16 keys read ahead in registers took 60 us (295 instructions a step, two thirds of
+// them not products), with a ring 52 us; 32 keys share the page lookups, maxima and rescaling (only where a maximum
+// moved).
 struct AttendParams {
     Kv8Params c;
     const uint16_t* q;
@@ -178,12 +186,24 @@ struct AttendParams {
 };
 
 constexpr int kAttWarps = 8;
+constexpr int kKeyRow = 64, kValueRow = 80;            // bytes: free of bank conflicts as the lanes read them
+constexpr int kStageBytes = 32 * (kKeyRow + kValueRow), kStages = 2;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 struct __align__(16) AttendShared {
     float o[16][kHeadDim + 4];
     float m[16], top[16], l[16];                       // running maxima (log2) and sum
 };
+
+static_assert(sizeof(AttendShared) <= kStages * kStageBytes, "the merge reuses the rings");
+constexpr int kAttShared = kAttWarps * kStages * kStageBytes;
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+    const uint32_t n = valid ? 16u : 0u;               // 0: the 16 bytes are zero-filled
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -228,11 +248,39 @@ __device__ __forceinline__ int load_q(const uint16_t* row, int t, uint32_t (&f)[
     return ex;
 }
 
-__global__ void __launch_bounds__(kAttWarps * 32) kv8_attend_kernel(AttendParams p) {
+// The running softmaxes of n parts, `kPer` dims of one row, in the order of the parts.
+template <int kPer> struct Merged {
+    float m, top, l, acc[kPer];
+    template <typename F> __device__ __forceinline__ void take(int n, int row, int d0, F&& part) {
+        m = top = kNegInf;
+        l = 0.f;
+        for (int i = 0; i < n; ++i) {
+            m = fmaxf(m, part(i)->m[row]);
+            top = fmaxf(top, part(i)->top[row]);
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+        for (int i = 0; i < n; ++i) {
+            const AttendShared* x = part(i);
+            if (x->l[row] == 0.f) continue;
+            l += x->l[row] * ex2(x->m[row] - m);
+            const float f = ex2(x->top[row] - top);
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) acc[k] += x->o[row][d0 + k] * f;
+        }
+    }
+};
+
+// kHalf: tiles of 8 rows (a decode step of up to 8 query heads per kv head): the lower half of the 16-row operand is
+// empty and its softmax is left out.
+template <bool kHalf>
+__global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_kernel(AttendParams p) {
+    constexpr int kRows = kHalf ? 8 : 16, kR = kHalf ? 1 : 2;              // rows of a tile, of a lane
     const Kv8Params& c = p.c;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    __shared__ AttendShared sh[kAttWarps];
+    extern __shared__ __align__(128) unsigned char smem[];
+    AttendShared* sh = reinterpret_cast<AttendShared*>(smem);              // after the loop, over the rings
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y, r = blockIdx.z;
     int first = r, count = 1;
@@ -244,110 +292,184 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv8_attend_kernel(AttendParams
     const int seq = max(c.seq_lens[r], 0);
     const long long capacity = (long long)c.bt_cols << c.page_shift;
     const int* table = c.block_table + r * c.bt_stride;
-    for (int tile = blockIdx.x / C; tile * 16 < rows; tile += p.tiles) {
-        // ---- the two rows of this lane
-        int len[2], ex[2];
-        uint32_t qa[2][8];
+    for (int tile = blockIdx.x / C; tile * kRows < rows; tile += p.tiles) {
+        // ---- keys: steps of 32 keys, a contiguous share per CTA, dealt to its warps
+        const int last = (min(tile * kRows + kRows, rows) - 1) / p.group, lead = tile * kRows / p.group;
+        const int len_max = (int)min((long long)max(seq - count + last + 1, 0), capacity);
+        const int len_min = (int)min((long long)max(seq - count + lead + 1, 0), capacity);
+        const int steps = (len_max + 31) / 32, share = (steps + C - 1) / C;
+        const int s_end = min((rank + 1) * share, steps);
+        // the pages of the halves of this warp's next 16 steps and their scales, one half per lane; kStages - 1 steps are
+        // on their way to shared memory while one is used
+        int pages = -1, old_pages = -1;
+        uint32_t scale2 = 0, old_scale2 = 0;                                 // E8M0 of K, of V
+        unsigned char* ring = smem + warp * kStages * kStageBytes;
+        long long lane_off = (lane >> 2) * c.token_stride + 16 * (lane & 3);
+        const uint8_t* k_lane = c.cache + (long long)h * c.head_stride + c.k_off + lane_off;
+        const long long v_from_k = c.v_off - c.k_off, eight = 8 * c.token_stride;
+        unsigned char* to_k = ring + (lane >> 2) * kKeyRow + 16 * (lane & 3);
+        unsigned char* to_v = ring + 32 * kKeyRow + (lane >> 2) * kValueRow + 16 * (lane & 3);
+        auto fetch = [&](int i) {                                            // this warp's i-th step
+            const int s = rank * share + warp + i * kAttWarps;
+            if ((i & 15) == 0) {
+                const int unit = 2 * (s + (lane >> 1) * kAttWarps) + (lane & 1);
+                old_pages = pages;
+                old_scale2 = scale2;
+                pages = unit < 2 * s_end && unit * 16 < len_max ? table[(unit * 16) >> c.page_shift] : -1;
+                if (pages >= c.pages || pages < 0) pages = -1;
+                scale2 = pages < 0 ? 0u : *reinterpret_cast<const uint16_t*>(c.scales + ((long long)pages * c.kv_heads + h) * 2);
+            }
+            const int page0 = __shfl_sync(kFullMask, pages, 2 * (i & 15)), page1 = __shfl_sync(kFullMask, pages, 2 * (i & 15) + 1);
+            if (s < s_end) {
+                const int at = (i % kStages) * kStageBytes;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = tile * 16 + g + 8 * i;
+                for (int u = 0; u < 2; ++u) {
+                    const int page = u ? page1 : page0, key0 = s * 32 + u * 16, left = page < 0 ? 0 : len_max - key0;
+                    const uint8_t* from = k_lane + (long long)max(page, 0) * c.page_stride +
+                                          (long long)(key0 & ((1 << c.page_shift) - 1)) * c.token_stride;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const bool on = (lane >> 2) + 8 * j < left;
+                        const uint8_t* src = on ? from + (j ? eight : 0) : k_lane - lane_off;
+                        cp_async16(to_k + at + (16 * u + 8 * j) * kKeyRow, src, on);
+                        cp_async16(to_v + at + (16 * u + 8 * j) * kValueRow, src + v_from_k, on);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll 1
+        for (int i = 0; i < kStages - 1; ++i) fetch(i);
+        // ---- the rows of this lane
+        int len[kR], ex[kR];
+        uint32_t qa[2][8] = {};
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+            const int row = tile * kRows + g + 8 * i;
             const int tok = row / p.group;
             const bool on = row < rows;
-            len[i] = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : 0;
+            len[i] = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : len_max;
             ex[i] = load_q(on ? p.q + (long long)(first + tok) * p.q_token + (long long)(h * p.group + row - tok * p.group) * p.q_head
                               : nullptr, t, qa[i]);
         }
-        const int last = (min(tile * 16 + 16, rows) - 1) / p.group, lead = tile * 16 / p.group;
-        const int len_max = (int)min((long long)max(seq - count + last + 1, 0), capacity);
-        const int len_min = tile * 16 + 16 > rows ? 0 : (int)min((long long)max(seq - count + lead + 1, 0), capacity);
-        const float qs[2] = {p.scale * exp2_biased(127 + ex[0]), p.scale * exp2_biased(127 + ex[1])};
-        // ---- keys: steps of 16 keys, a contiguous share per CTA, dealt to its warps
-        const int steps = (len_max + 15) / 16, share = (steps + C - 1) / C;
-        const int s_end = min((rank + 1) * share, steps);
-        float o[8][4], m[2] = {kNegInf, kNegInf}, top[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+        float qs[kR];
+#pragma unroll
+        for (int i = 0; i < kR; ++i) qs[i] = p.scale * exp2_biased(127 + ex[i]);
+        float o[8][4], m[kR], top[kR], l[kR];
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+            m[i] = top[i] = kNegInf;
+            l[i] = 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        for (int st = rank * share + warp; st < s_end; st += kAttWarps) {
-            const int key0 = st * 16;
-            const int page = table[key0 >> c.page_shift];
-            if (page < 0 || page >= c.pages) continue;                       // masked
-            const uint8_t* base = c.cache + (long long)page * c.page_stride + (long long)h * c.head_stride +
-                                  (long long)(key0 & ((1 << c.page_shift) - 1)) * c.token_stride;
-            const uint8_t* sc = c.scales + ((long long)page * c.kv_heads + h) * 2;
-            const uint32_t ek = sc[0];
-            const int ev = (int)sc[1] - 127;
-            uint4 kw[2] = {};
-            uint2 vw[4] = {};
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (key0 + g + 8 * j < len_max)
-                    kw[j] = *reinterpret_cast<const uint4*>(base + c.k_off + (g + 8 * j) * c.token_stride + 16 * t);
+        for (int i = 0, st = rank * share + warp; st < s_end; ++i, st += kAttWarps) {
+            __syncwarp();                                                    // the stage that is refilled has been read
+            fetch(i + kStages - 1);
+            // the step's scales; the lanes may already hold the next 16 steps
+            const bool older = ((i + kStages - 1) & ~15) != (i & ~15);
+            const int mine_pages = older ? old_pages : pages;
+            const uint32_t mine_scale2 = older ? old_scale2 : scale2;
+            const bool valid[2] = {__shfl_sync(kFullMask, mine_pages, 2 * (i & 15)) >= 0,
+                                   __shfl_sync(kFullMask, mine_pages, 2 * (i & 15) + 1) >= 0};
+            const uint32_t sc[2] = {__shfl_sync(kFullMask, mine_scale2, 2 * (i & 15)),
+                                    __shfl_sync(kFullMask, mine_scale2, 2 * (i & 15) + 1)};
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            const unsigned char* from = ring + (i % kStages) * kStageBytes;
+            float s[4][4] = {};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int key = 2 * t + (j & 1) + 8 * (j >> 1);
-                if (key0 + key < len_max)
-                    vw[j] = *reinterpret_cast<const uint2*>(base + c.v_off + key * c.token_stride + 8 * g);
-            }
-            float s[2][4] = {};
+                const uint4 kw = *reinterpret_cast<const uint4*>(from + (g + 8 * j) * kKeyRow + 16 * t);
+                const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_f16(s[j], qa[0][2 * k], qa[1][2 * k], qa[0][2 * k + 1], qa[1][2 * k + 1],
-                            e4m3x2_to_f16x2(w[k] & 0xffffu), e4m3x2_to_f16x2(w[k] >> 16));
-            }
-            const float ks = exp2_biased(ek);
-            const bool edge = key0 + 16 > len_min;
-            float mx[2] = {kNegInf, kNegInf};
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 8 * j + 2 * t + (i & 1);
-                    s[j][i] = s[j][i] * ks * qs[i >> 1];
-                    if (edge && key >= len[i >> 1]) s[j][i] = kNegInf;
-                    mx[i >> 1] = fmaxf(mx[i >> 1], s[j][i]);
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t lo, hi;
+                    e4m3x4_to_f16(w[k], lo, hi);
+                    mma_f16(s[j], qa[0][2 * k], qa[1][2 * k], qa[0][2 * k + 1], qa[1][2 * k + 1], lo, hi);
                 }
-            float pw[2][4];
-            float turn[2];
+            }
+            const bool edge = st * 32 + 32 > len_min || !valid[0] || !valid[1];
+            const float ev[2] = {(float)(int)(sc[0] >> 8) - 127.f, (float)(int)(sc[1] >> 8) - 127.f};
+            const float ks[2] = {exp2_biased(sc[0] & 0xffu), exp2_biased(sc[1] & 0xffu)};
+            float pw[4][4] = {}, turn[kR];
+            bool turned = false;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                mx[i] = quad_max(mx[i]);
-                const float m1 = fmaxf(m[i], mx[i]), t1 = fmaxf(top[i], mx[i] + (float)ev);
-                const float mu = m1 == kNegInf ? 0.f : m1, tu = t1 == kNegInf ? 0.f : t1;
-                l[i] *= ex2(m[i] - mu);
-                turn[i] = ex2(top[i] - tu);
-                const float f = ex2(fminf(mu + (float)ev - tu, 127.f));      // 2^(s - m) -> 2^(s + ev - top)
+            for (int i2 = 0; i2 < kR; ++i2) {
+                float mx[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int u = 0; u < 2; ++u) {
+                    const float f0 = ks[u] * qs[i2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float e = ex2(s[j][2 * i + k] - mu);
-                        l[i] += e;
-                        pw[j][2 * i + k] = e * f;
+                    for (int j = 2 * u; j < 2 * u + 2; ++j)
+#pragma unroll
+                        for (int k = 2 * i2; k < 2 * i2 + 2; ++k) s[j][k] *= f0;
+                    if (edge) {
+                        const int limit = valid[u] ? len[i2] - st * 32 - 2 * t : 0;      // keys from here on are masked
+#pragma unroll
+                        for (int j = 2 * u; j < 2 * u + 2; ++j)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                if (8 * j + k >= limit || !valid[u]) s[j][2 * i2 + k] = kNegInf;
                     }
-                m[i] = m1;
-                top[i] = t1;
-            }
-            const uint32_t a0 = pack_f16x2(pw[0][0], pw[0][1]), a1 = pack_f16x2(pw[0][2], pw[0][3]);
-            const uint32_t a2 = pack_f16x2(pw[1][0], pw[1][1]), a3 = pack_f16x2(pw[1][2], pw[1][3]);
+                    mx[u] = quad_max(fmaxf(fmaxf(s[2 * u][2 * i2], s[2 * u][2 * i2 + 1]), fmaxf(s[2 * u + 1][2 * i2], s[2 * u + 1][2 * i2 + 1])));
+                }
+                const float m1 = fmaxf(m[i2], fmaxf(mx[0], mx[1])), t1 = fmaxf(top[i2], fmaxf(mx[0] + ev[0], mx[1] + ev[1]));
+                const float mu = m1 == kNegInf ? 0.f : m1, tu = t1 == kNegInf ? 0.f : t1;
+                l[i2] *= ex2(m[i2] - mu);
+                turn[i2] = ex2(top[i2] - tu);
+                turned |= t1 > top[i2];
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                o[d][0] *= turn[0]; o[d][1] *= turn[0]; o[d][2] *= turn[1]; o[d][3] *= turn[1];
+                for (int u = 0; u < 2; ++u) {
+                    const float f = ex2(fminf(mu + ev[u] - tu, 127.f));      // 2^(s - m) -> 2^(s + ev - top)
+#pragma unroll
+                    for (int j = 2 * u; j < 2 * u + 2; ++j)
+#pragma unroll
+                        for (int k = 2 * i2; k < 2 * i2 + 2; ++k) {
+                            const float e = ex2(s[j][k] - mu);
+                            l[i2] += e;
+                            pw[j][k] = e * f;
+                        }
+                }
+                m[i2] = m1;
+                top[i2] = t1;
+            }
+            if (__any_sync(kFullMask, turned)) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+#pragma unroll
+                    for (int i2 = 0; i2 < kR; ++i2) {
+                        o[d][2 * i2] *= turn[i2];
+                        o[d][2 * i2 + 1] *= turn[i2];
+                    }
             }
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {                                    // dims 8g + 2d, 8g + 2d + 1
-                const uint32_t sel = (d & 1) ? 0x7362u : 0x5140u;
-                const uint32_t lo = __byte_perm(d < 2 ? vw[0].x : vw[0].y, d < 2 ? vw[1].x : vw[1].y, sel);
-                const uint32_t hi = __byte_perm(d < 2 ? vw[2].x : vw[2].y, d < 2 ? vw[3].x : vw[3].y, sel);
-                mma_f16(o[2 * d], a0, a1, a2, a3, e4m3x2_to_f16x2(lo & 0xffffu), e4m3x2_to_f16x2(hi & 0xffffu));
-                mma_f16(o[2 * d + 1], a0, a1, a2, a3, e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi >> 16));
+            for (int u = 0; u < 2; ++u) {
+                uint2 vw[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    vw[j] = *reinterpret_cast<const uint2*>(from + 32 * kKeyRow + (16 * u + 2 * t + (j & 1) + 8 * (j >> 1)) * kValueRow + 8 * g);
+                const uint32_t a0 = pack_f16x2(pw[2 * u][0], pw[2 * u][1]), a1 = kHalf ? 0u : pack_f16x2(pw[2 * u][2], pw[2 * u][3]);
+                const uint32_t a2 = pack_f16x2(pw[2 * u + 1][0], pw[2 * u + 1][1]),
+                               a3 = kHalf ? 0u : pack_f16x2(pw[2 * u + 1][2], pw[2 * u + 1][3]);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {                                // dims 8g + 2d, 8g + 2d + 1
+                    const uint32_t sel = (d & 1) ? 0x7362u : 0x5140u;
+                    const uint32_t lo = __byte_perm(d < 2 ? vw[0].x : vw[0].y, d < 2 ? vw[1].x : vw[1].y, sel);
+                    const uint32_t hi = __byte_perm(d < 2 ? vw[2].x : vw[2].y, d < 2 ? vw[3].x : vw[3].y, sel);
+                    uint32_t b00, b01, b10, b11;
+                    e4m3x4_to_f16(lo, b00, b10);
+                    e4m3x4_to_f16(hi, b01, b11);
+                    mma_f16(o[2 * d], a0, a1, a2, a3, b00, b01);
+                    mma_f16(o[2 * d + 1], a0, a1, a2, a3, b10, b11);
+                }
             }
         }
         // ---- merge the warps, then the CTAs
+        cp_async_wait<0>();
+        __syncthreads();                                                     // the rings are read: their memory is the merge's now
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kR; ++i) {
             l[i] += __shfl_xor_sync(kFullMask, l[i], 1);
             l[i] += __shfl_xor_sync(kFullMask, l[i], 2);
             const int row = g + 8 * i;
@@ -363,49 +485,32 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv8_attend_kernel(AttendParams
             }
         }
         __syncthreads();
-        const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;       // 16 threads per row, 4 dims each
-        auto merge = [&](int n, auto&& part, float& M, float& TOP, float& L, float (&acc)[4]) {
-            M = TOP = kNegInf;
-            L = 0.f;
-            for (int i = 0; i < n; ++i) {
-                M = fmaxf(M, part(i).m[row]);
-                TOP = fmaxf(TOP, part(i).top[row]);
-            }
-            acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-            for (int i = 0; i < n; ++i) {
-                const AttendShared& x = part(i);
-                if (x.l[row] == 0.f) continue;
-                L += x.l[row] * ex2(x.m[row] - M);
-                const float f = ex2(x.top[row] - TOP);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] += x.o[row][d0 + k] * f;
-            }
-        };
-        float M, TOP, L, acc[4];
-        merge(kAttWarps, [&](int i) -> const AttendShared& { return sh[i]; }, M, TOP, L, acc);
+        constexpr int kPer = kRows * kHeadDim / (kAttWarps * 32);            // dims of one row that a thread merges: 2, 4 or 8
+        const int row = (int)threadIdx.x / (kHeadDim / kPer), d0 = (int)threadIdx.x % (kHeadDim / kPer) * kPer;
+        Merged<kPer> a;
+        a.take(kAttWarps, row, d0, [&](int i) { return &sh[i]; });
         if (C > 1) {
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sh[0].o[row][d0 + k] = acc[k];
+            for (int k = 0; k < kPer; ++k) sh[0].o[row][d0 + k] = a.acc[k];
             if (d0 == 0) {
-                sh[0].m[row] = M;
-                sh[0].top[row] = TOP;
-                sh[0].l[row] = L;
+                sh[0].m[row] = a.m;
+                sh[0].top[row] = a.top;
+                sh[0].l[row] = a.l;
             }
             cluster.sync();
             if (rank == 0)
-                merge(C, [&](int i) -> const AttendShared& { return *cluster.map_shared_rank(&sh[0], i); }, M, TOP, L, acc);
+                a.take(C, row, d0, [&](int i) { return cluster.map_shared_rank(&sh[0], i); });
         }
-        const int at = tile * 16 + row;
+        const int at = tile * kRows + row;
         if (rank == 0 && at < rows) {
             const int tok = at / p.group, head = h * p.group + at - tok * p.group;
-            const float f = L == 0.f ? 0.f : ex2(TOP - M) / L;
-            uint2 w;
-            w.x = pack_bf16x2(acc[0] * f, acc[1] * f);
-            w.y = pack_bf16x2(acc[2] * f, acc[3] * f);
-            *reinterpret_cast<uint2*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head + d0) = w;
+            const float f = a.l == 0.f ? 0.f : ex2(a.top - a.m) / a.l;
+            uint32_t* to = reinterpret_cast<uint32_t*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head + d0);
+#pragma unroll
+            for (int k = 0; k < kPer; k += 2) to[k / 2] = pack_bf16x2(a.acc[k] * f, a.acc[k + 1] * f);
             if (p.lse && d0 == 0)
-                p.lse[(long long)(first + tok) * p.q_heads + head] = L == 0.f ? kNegInf : (M + log2f(L)) * 0.6931471805599453f;
+                p.lse[(long long)(first + tok) * p.q_heads + head] = a.l == 0.f ? kNegInf : (a.m + log2f(a.l)) * 0.6931471805599453f;
         }
         if (C > 1) cluster.sync(); else __syncthreads();                     // the parts are read before they are written again
     }
@@ -484,15 +589,25 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     p.scale = scale * 1.4426950408889634f;
     int longest = p.c.cu ? (max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens) : 1;
     if ((long long)longest * p.group > 0x7fffffffLL - 16) return kErrShape;
-    const long long tiles = ((long long)longest * p.group + 15) / 16;
+    const int tile_rows = (long long)longest * p.group <= 8 ? 8 : 16;
+    const long long tiles = ((long long)longest * p.group + tile_rows - 1) / tile_rows;
     const long long items = tiles * p.c.kv_heads * p.c.batch;
-    const long long steps = (((long long)p.c.bt_cols << p.c.page_shift) + 15) / 16;
-    int c = 1;
-    while (c < 8 && items * c < 296 && steps > 2 * kAttWarps * c) c *= 2;
+    const long long steps = (((long long)p.c.bt_cols << p.c.page_shift) + 31) / 32;
+    // CTAs that share the keys of one item: as many as are resident at once (two on each of 148 SMs), at least two steps
+    // for each warp.  Where that leaves eight steps or more an eighth more CTAs is worth a second wave (32 requests x 5 kv
+    // heads at 8192 keys: 27.7 us with two CTAs an item, 38.9 with one); with two steps it is not (16 requests at 2048
+    // keys: 13.1 us with four, 10.0 with three).  Fewer than two steps cost more in merging than they save (8 requests of
+    // 5 tokens at 2047 keys: 12.3 us, 9.4).
+    const long long worth = steps / (2 * kAttWarps);
+    long long fit = 340 / items;
+    if (fit > steps / (8 * kAttWarps)) fit = 296 / items;
+    const long long share = fit < worth ? fit : worth;
+    const int c = (int)(share < 1 ? 1 : (share < 8 ? share : 8));
     p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p.tiles * c), (unsigned)p.c.kv_heads, (unsigned)p.c.batch);
     cfg.blockDim = dim3(kAttWarps * 32);
+    cfg.dynamicSmemBytes = kAttShared;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -500,5 +615,7 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kv8_attend_kernel, p);
+    const auto kernel = tile_rows == 8 ? kv8_attend_kernel<true> : kv8_attend_kernel<false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttShared);
+    return (int)(e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, p));
 }
