@@ -213,6 +213,10 @@ int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long long q_token_s
                      long long out_token_stride, long long out_head_stride, void* lse, int tokens, int q_heads,
                      int max_query_len, float scale, void* stream);
 
+/* Bounded barrier waits of the kernel for many query tokens that expired since load (0 = healthy; -1 = CUDA error).
+ * Synchronises. */
+long long pk_kv8_wait_timeouts(void);
+
 /* ---------------------------------------------------------------- sampling */
 
 /* Draw one token per row of logits [rows, vocab] (dtype 0 bf16, 1 fp16, 2 fp32; row_stride in elements; vocab <= 262144)

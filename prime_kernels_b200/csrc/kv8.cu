@@ -516,6 +516,405 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
     }
 }
 
+// ---------------------------------------------------------------- attention of many query tokens (prompt chunks)
+// The same rows and the same arithmetic with 128 rows a tile, on tcgen05: S = Q K^T (M 128, N 64, both operands K-major
+// in shared memory) and O += P V (P from tensor memory, V as it lies: [key][dim], MN-major), accumulators in tensor
+// memory.  One CTA holds one tile; warps 0-3 own a row a thread (softmax), warps 4-5 turn e4m3 pages into swizzled f16
+// tiles of 64 keys, one thread of warp 6 issues the products (eight warps, so that a thread may have 128 registers).  S is double-buffered, so the next scores are computed
+// while the softmax works, and two CTAs share an SM (256 columns of tensor memory each), so one's products run under
+// the other's exponentials.
+//
+// Bound by the exponentials: 16 a clock and SM against 64 x 4 flops each, a quarter of the tensor peak at head dim 64.
+// `top` is raised only where a row's maximum has grown by 2^8, so that the accumulator is rarely rescaled; f16 holds 2^8
+// times the weights.
+constexpr int kTileRows = 128, kTileKeys = 64, kPromptStages = 3;
+constexpr int kPromptThreads = 256, kProducers = 64, kRowsEach = kTileKeys * 4 / kProducers;   // 16-byte parts of K rows a producer carries
+constexpr uint32_t kPromptCols = 256, kColP = 128, kColO = 192;            // S in columns 0..127, P in 128..191, two of each
+constexpr float kLazy = 8.f;
+#ifndef PK_MINROWS
+#define PK_MINROWS 64
+#endif
+constexpr int kPromptMinRows = PK_MINROWS;
+
+struct PromptShared {
+    uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full, pv_done[2], drain;
+    float ks[kPromptStages][4], ev[kPromptStages][4], bias[kPromptStages][4];   // per 16 keys; bias -inf: no page
+    uint32_t tmem;
+    volatile int abort;
+};
+constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + (int)sizeof(PromptShared);
+
+__device__ unsigned int g_kv8_wait_timeouts;
+
+// Bounded wait: gives up after some seconds, or as soon as another thread of the CTA has.
+__device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
+    for (uint32_t n = 0; n < (1u << 20); ++n) {
+        if (mbar_test(bar, parity & 1u)) return;
+        if ((n & 63) == 63 && sh.abort) return;
+    }
+    if (!sh.abort) {
+        sh.abort = 1;
+        atomicAdd(&g_kv8_wait_timeouts, 1u);
+    }
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 128-byte swizzle, rows of 128 bytes, 1024 bytes from one group of eight rows to the next, descriptor version 1; the same
+// for a K-major operand (row = M or N index) and an MN-major one of 64 elements (row = K index)
+__device__ __forceinline__ uint64_t tile_desc(const void* p) {
+    return (((uint64_t)smem_u32(p) >> 4) & 0x3fffull) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f16 x f16 -> f32, M 128, N 64; bit 16: B is MN-major
+constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kTileKeys >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const float* v) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+        "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+        "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendParams p) {
+    const Kv8Params& c = p.c;
+    extern __shared__ unsigned char raw[];
+    unsigned char* q_tile = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* kv_tiles = q_tile + kTileRows * 128;                    // per stage: K, V
+    PromptShared& sh = *reinterpret_cast<PromptShared*>(kv_tiles + kPromptStages * 2 * kTileKeys * 128);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.y, r = blockIdx.z;
+    int first = r, count = 1;
+    if (c.cu) {
+        first = max(c.cu[r], 0);
+        count = min(c.cu[r + 1], c.tokens) - first;
+    }
+    const int rows = count * p.group;
+    const int tile0 = p.tiles - 1 - (int)blockIdx.x;                       // later tiles see more keys: they start first
+    if (tile0 * kTileRows >= rows) return;                                 // the whole CTA
+    const int seq = max(c.seq_lens[r], 0);
+    const long long capacity = (long long)c.bt_cols << c.page_shift;
+    const int* table = c.block_table + r * c.bt_stride;
+
+    if (tid == 0) {
+        for (int i = 0; i < kPromptStages; ++i) {
+            mbar_init(&sh.full[i], kProducers);
+            mbar_init(&sh.empty[i], 1);
+        }
+        mbar_init(&sh.q_full, 128);
+        mbar_init(&sh.s_full[0], 1);
+        mbar_init(&sh.s_full[1], 1);
+        mbar_init(&sh.p_full, 128);
+        mbar_init(&sh.pv_done[0], 1);
+        mbar_init(&sh.pv_done[1], 1);
+        mbar_init(&sh.drain, 1);
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 6) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(kPromptCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    uint32_t n = 0, tiles_done = 0;                                        // steps and tiles before this tile: barrier parities
+    for (int tile = tile0; tile * kTileRows < rows; tile += p.tiles, ++tiles_done) {
+        const int last = (min(tile * kTileRows + kTileRows, rows) - 1) / p.group, lead = tile * kTileRows / p.group;
+        const int len_max = (int)min((long long)max(seq - count + last + 1, 0), capacity);
+        const int len_min = (int)min((long long)max(seq - count + lead + 1, 0), capacity);
+        const int steps = (len_max + kTileKeys - 1) / kTileKeys;
+        if (warp < 4) {
+            // ---------------- softmax: one row a thread
+            const int row = tile * kTileRows + tid, tok = row / p.group, head = h * p.group + row - tok * p.group;
+            const bool on = row < rows;
+            const int len = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : len_max;
+            float qs;
+            {
+                uint4 w[8];
+                const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(first + tok) * p.q_token + (long long)head * p.q_head);
+                float amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = on ? src[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(bf16_lo(u[j])), fabsf(bf16_hi(u[j]))));
+                }
+                const int ex = max(min((int)(__float_as_uint(amax) >> 23) - 134, 126), -126);
+                const float f2 = copysignf(exp2_biased(127 - ex), p.scale);
+                qs = fabsf(p.scale) * exp2_biased(127 + ex);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                    uint32_t f[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[j] = pack_f16x2(bf16_lo(u[j]) * f2, bf16_hi(u[j]) * f2);
+                    *reinterpret_cast<uint4*>(q_tile + tid * 128 + ((i ^ (tid & 7)) * 16)) = make_uint4(f[0], f[1], f[2], f[3]);
+                }
+                fence_async_smem();
+                mbar_arrive(&sh.q_full);
+            }
+            const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+            float m = kNegInf, top = kNegInf, l = 0.f;
+            for (int i = 0; i < steps; ++i) {
+                const uint32_t at = n + i, stage = at % kPromptStages;
+                prompt_wait(sh, &sh.full[stage], at / kPromptStages);      // the scales are there
+                prompt_wait(sh, &sh.s_full[at & 1], at >> 1);
+                tc_fence_after();
+                // 32 scores at a time, read twice: all 64 of them and their weights do not fit the registers
+                float s[32];
+                auto half = [&](int d) {
+                    tmem_ld32(lanes + (at & 1) * kTileKeys + 32 * d, s);
+                    tmem_ld_wait();
+                    const int left = len - i * kTileKeys - 32 * d;         // scores from here on are masked
+                    if (i * kTileKeys + kTileKeys > len_min) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (k >= left) s[k] = kNegInf;
+                    }
+                };
+                float ck[4], m1 = m, t1 = top;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    half(d);
+#pragma unroll
+                    for (int u = 2 * d; u < 2 * d + 2; ++u) {
+                        float mx = s[16 * (u & 1)];
+#pragma unroll
+                        for (int k = 1; k < 16; ++k) mx = fmaxf(mx, s[16 * (u & 1) + k]);
+                        ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);       // never 0: a masked score times it stays -inf
+                        mx = fmaf(mx, ck[u], sh.bias[stage][u]);
+                        m1 = fmaxf(m1, mx);
+                        t1 = fmaxf(t1, mx + sh.ev[stage][u]);
+                    }
+                }
+                const float mu = m1 == kNegInf ? 0.f : m1;
+                l *= ex2(m - mu);
+                m = m1;
+                float turn = 1.f;
+                if (t1 > top + kLazy) {                                    // top = -inf: any finite maximum
+                    turn = ex2(top - t1);
+                    top = t1;
+                }
+                const float tu = top == kNegInf ? 0.f : top;
+                if (i > 1) {                                               // this P has been read
+                    prompt_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
+                    tc_fence_after();
+                }
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    half(d);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int u = 2 * d; u < 2 * d + 2; ++u) {
+                        const float f = ex2(fminf(mu + sh.ev[stage][u] - tu, 127.f));
+                        const float shift = sh.bias[stage][u] - mu;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            const float a = ex2(fmaf(s[16 * (u & 1) + k], ck[u], shift)), b = ex2(fmaf(s[16 * (u & 1) + k + 1], ck[u], shift));
+                            sum += a + b;
+                            pk[8 * (u & 1) + k / 2] = pack_f16x2(a * f, b * f);
+                        }
+                        l += sum;
+                    }
+                    tmem_st16(lanes + kColP + (at & 1) * 32 + 16 * d, pk);
+                }
+                if (i > 0 && __any_sync(kFullMask, turn != 1.f)) {
+                    prompt_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        tmem_ld32(lanes + kColO + 32 * d, s);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[k] *= turn;
+                        tmem_st32(lanes + kColO + 32 * d, s);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&sh.p_full);
+            }
+            float f = 0.f;
+            if (steps > 0) {
+                prompt_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1);
+                tc_fence_after();
+                f = l == 0.f ? 0.f : ex2(top - m) / l;
+            }
+            uint4* to = reinterpret_cast<uint4*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                float o[32];
+                if (steps > 0) {
+                    tmem_ld32(lanes + kColO + 32 * d, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = f == 0.f ? 0.f : o[k] * f;
+                if (on) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        to[4 * d + k] = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]),
+                                                   pack_bf16x2(o[8 * k + 4], o[8 * k + 5]), pack_bf16x2(o[8 * k + 6], o[8 * k + 7]));
+                }
+            }
+            if (on && p.lse) p.lse[(long long)(first + tok) * p.q_heads + head] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
+            tc_fence_before();                                             // the accumulator is read: the next tile may write it
+        } else if (warp < 6) {
+            // ---------------- e4m3 pages to f16 tiles: a thread carries 16 bytes of kRowsEach K rows and as many V rows
+            const int pid = tid - 128, key = pid >> 2, part = pid & 3;
+            constexpr int kApart = kProducers / 4;                         // rows between a thread's
+            const uint8_t* from = c.cache + (long long)h * c.head_stride + 16 * part;
+            const uint8_t* scales = c.scales + 2 * h;
+            uint4 kq[kRowsEach], vq[kRowsEach];
+            int page[kRowsEach], group_page = -1;                          // of the step after the one in kq, vq
+            uint32_t sc = 0;                                               // scales of 16 keys; 0xffffffff: no page
+            auto page_of = [&](int at) {
+                if (at >= len_max) return -1;
+                const int page = table[at >> c.page_shift];
+                return page < c.pages ? page : -1;
+            };
+            auto look_up = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < kRowsEach; ++j) page[j] = page_of(i * kTileKeys + key + kApart * j);
+                if (pid < 4) group_page = page_of(i * kTileKeys + 16 * pid);
+            };
+            auto load = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < kRowsEach; ++j) {
+                    const int at = i * kTileKeys + key + kApart * j;
+                    const bool live = page[j] >= 0 && at < len_max;
+                    const uint8_t* src = from + (long long)page[j] * c.page_stride +
+                                         (long long)(at & ((1 << c.page_shift) - 1)) * c.token_stride;
+                    kq[j] = live ? ld_stream_16(src + c.k_off) : make_uint4(0, 0, 0, 0);
+                    vq[j] = live ? ld_stream_16(src + c.v_off) : make_uint4(0, 0, 0, 0);
+                }
+                if (pid < 4)
+                    sc = group_page < 0 ? 0xffffffffu
+                                        : *reinterpret_cast<const uint16_t*>(scales + (long long)group_page * c.kv_heads * 2);
+            };
+            look_up(0);
+            load(0);
+            look_up(1);
+            for (int i = 0; i < steps; ++i) {
+                const uint32_t at = n + i, stage = at % kPromptStages;
+                if (at >= kPromptStages) prompt_wait(sh, &sh.empty[stage], at / kPromptStages - 1);
+                unsigned char* k_tile = kv_tiles + stage * 2 * kTileKeys * 128;
+#pragma unroll
+                for (int j = 0; j < kRowsEach; ++j) {
+                    const int row = key + kApart * j;
+                    unsigned char* to = k_tile + row * 128;
+                    const uint32_t a = ((2 * part) ^ (row & 7)) * 16, b = ((2 * part + 1) ^ (row & 7)) * 16;
+                    uint4 lo, hi;
+                    e4m3x4_to_f16(kq[j].x, lo.x, lo.y);
+                    e4m3x4_to_f16(kq[j].y, lo.z, lo.w);
+                    e4m3x4_to_f16(kq[j].z, hi.x, hi.y);
+                    e4m3x4_to_f16(kq[j].w, hi.z, hi.w);
+                    *reinterpret_cast<uint4*>(to + a) = lo;
+                    *reinterpret_cast<uint4*>(to + b) = hi;
+                    e4m3x4_to_f16(vq[j].x, lo.x, lo.y);
+                    e4m3x4_to_f16(vq[j].y, lo.z, lo.w);
+                    e4m3x4_to_f16(vq[j].z, hi.x, hi.y);
+                    e4m3x4_to_f16(vq[j].w, hi.z, hi.w);
+                    *reinterpret_cast<uint4*>(to + kTileKeys * 128 + a) = lo;
+                    *reinterpret_cast<uint4*>(to + kTileKeys * 128 + b) = hi;
+                }
+                const uint32_t scale2 = sc;
+                if (i + 1 < steps) {
+                    load(i + 1);
+                    look_up(i + 2);
+                }
+                if (pid < 4) {
+                    const bool none = scale2 == 0xffffffffu;
+                    sh.ks[stage][pid] = none ? 0.f : exp2_biased(scale2 & 0xffu);
+                    sh.ev[stage][pid] = none ? 0.f : (float)(int)(scale2 >> 8) - 127.f;
+                    sh.bias[stage][pid] = none ? kNegInf : 0.f;
+                }
+                fence_async_smem();
+                mbar_arrive(&sh.full[stage]);
+            }
+        } else if (warp == 6 && lane == 0) {
+            // ---------------- products
+            prompt_wait(sh, &sh.q_full, tiles_done);
+            const uint64_t dq = tile_desc(q_tile);
+            auto scores = [&](int i) {
+                const uint32_t at = n + i, stage = at % kPromptStages;
+                prompt_wait(sh, &sh.full[stage], at / kPromptStages);
+                tc_fence_after();
+                const uint64_t dk = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)                                // 16 dims = 32 bytes a product
+                    mma_ss(tmem + (at & 1) * kTileKeys, dq + 2 * k, dk + 2 * k, kIdescQK, k > 0);
+                mma_commit(&sh.s_full[at & 1]);
+            };
+            if (steps > 0) scores(0);
+            for (int i = 0; i < steps; ++i) {
+                const uint32_t at = n + i, stage = at % kPromptStages;
+                if (i + 1 < steps) scores(i + 1);
+                prompt_wait(sh, &sh.p_full, at);
+                tc_fence_after();
+                const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)                                // 16 keys = 2048 bytes of V, 8 columns of P
+                    mma_ts(tmem + kColO, tmem + kColP + (at & 1) * 32 + 8 * k, dv + 128 * k, kIdescPV, i > 0 || k > 0);
+                mma_commit(&sh.empty[stage]);
+                mma_commit(&sh.pv_done[at & 1]);
+            }
+        }
+        n += (uint32_t)steps;
+    }
+    if (warp == 6) {
+        if (lane == 0) {                                                   // nothing is in flight when the memory goes
+            mma_commit(&sh.drain);
+            prompt_wait(sh, &sh.drain, 0);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 6) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPromptCols) : "memory");
+}
+
 // ---------------------------------------------------------------- host
 int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     if (!a) return kErrNull;
@@ -546,6 +945,14 @@ int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
 }
 
 }  // namespace pk
+
+// Bounded waits of the prompt kernel that gave up since the library was loaded (0 in normal operation; a launch that
+// counted one produced invalid output).  Synchronises the device.
+extern "C" long long pk_kv8_wait_timeouts(void) {
+    unsigned int n = 0;
+    if (cudaMemcpyFromSymbol(&n, pk::g_kv8_wait_timeouts, sizeof(n)) != cudaSuccess) return -1;
+    return (long long)n;
+}
 
 extern "C" int pk_kv8_append(const PkKv8Cache* cache, const void* k, long long k_token_stride, long long k_head_stride,
                              const void* v, long long v_token_stride, long long v_head_stride, int tokens, void* stream) {
@@ -589,6 +996,17 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     p.scale = scale * 1.4426950408889634f;
     int longest = p.c.cu ? (max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens) : 1;
     if ((long long)longest * p.group > 0x7fffffffLL - 16) return kErrShape;
+    // rows a request is expected to have: the longest where the caller knows it, else the mean
+    const long long expected = (max_query_len > 0 || !p.c.cu ? (long long)longest : ((long long)tokens + p.c.batch - 1) / p.c.batch) * p.group;
+    if (expected >= kPromptMinRows) {
+        const long long tiles = ((long long)longest * p.group + kTileRows - 1) / kTileRows;
+        p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
+        const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptBytes);
+        if (e != cudaSuccess) return (int)e;
+        kv8_prompt_kernel<<<dim3((unsigned)p.tiles, (unsigned)p.c.kv_heads, (unsigned)p.c.batch), kPromptThreads, kPromptBytes,
+                            static_cast<cudaStream_t>(stream)>>>(p);
+        return (int)cudaPeekAtLastError();
+    }
     const int tile_rows = (long long)longest * p.group <= 8 ? 8 : 16;
     const long long tiles = ((long long)longest * p.group + tile_rows - 1) / tile_rows;
     const long long items = tiles * p.c.kv_heads * p.c.batch;
