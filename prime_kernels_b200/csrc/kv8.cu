@@ -210,6 +210,25 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+        "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
     asm volatile(
@@ -528,7 +547,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
 // `top` is raised only where a row's maximum has grown by 2^8, so that the accumulator is rarely rescaled; f16 holds 2^8
 // times the weights.
 constexpr int kTileRows = 128, kTileKeys = 64, kPromptStages = 3;
-constexpr int kPromptThreads = 256, kProducers = 64, kRowsEach = kTileKeys * 4 / kProducers;   // 16-byte parts of K rows a producer carries
+constexpr int kRawStages = 4, kRawBytes = kTileKeys * 128;              // e4m3 on its way
+constexpr int kPromptThreads = 256, kProducers = 64;
 constexpr uint32_t kPromptCols = 256, kColP = 128, kColO = 192;            // S in columns 0..127, P in 128..191, two of each
 constexpr float kLazy = 8.f;
 #ifndef PK_MINROWS
@@ -537,12 +557,12 @@ constexpr float kLazy = 8.f;
 constexpr int kPromptMinRows = PK_MINROWS;
 
 struct PromptShared {
-    uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full, pv_done[2], drain;
+    uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full[2], pv_done[2], drain;
     float ks[kPromptStages][4], ev[kPromptStages][4], bias[kPromptStages][4];   // per 16 keys; bias -inf: no page
     uint32_t tmem;
     volatile int abort;
 };
-constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + (int)sizeof(PromptShared);
+constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + kRawStages * kRawBytes + (int)sizeof(PromptShared);
 
 __device__ unsigned int g_kv8_wait_timeouts;
 
@@ -556,6 +576,11 @@ __device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uin
         sh.abort = 1;
         atomicAdd(&g_kv8_wait_timeouts, 1u);
     }
+}
+// The same for a whole warp whose next instruction is a warp-wide one: lanes may leave the polling loop apart.
+__device__ __forceinline__ void warp_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
+    prompt_wait(sh, bar, parity);
+    __syncwarp();
 }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -590,7 +615,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const float* v) {
+template <typename T> __device__ __forceinline__ void tmem_st32(uint32_t at, const T* v) {
     const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -601,13 +626,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const float* v) {
         "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* u) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
-        ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(at)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -616,7 +634,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
     extern __shared__ unsigned char raw[];
     unsigned char* q_tile = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* kv_tiles = q_tile + kTileRows * 128;                    // per stage: K, V
-    PromptShared& sh = *reinterpret_cast<PromptShared*>(kv_tiles + kPromptStages * 2 * kTileKeys * 128);
+    unsigned char* raw_ring = kv_tiles + kPromptStages * 2 * kTileKeys * 128;
+    PromptShared& sh = *reinterpret_cast<PromptShared*>(raw_ring + kRawStages * kRawBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.y, r = blockIdx.z;
     int first = r, count = 1;
@@ -639,7 +658,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
         mbar_init(&sh.q_full, 128);
         mbar_init(&sh.s_full[0], 1);
         mbar_init(&sh.s_full[1], 1);
-        mbar_init(&sh.p_full, 128);
+        mbar_init(&sh.p_full[0], 128);
+        mbar_init(&sh.p_full[1], 128);
         mbar_init(&sh.pv_done[0], 1);
         mbar_init(&sh.pv_done[1], 1);
         mbar_init(&sh.drain, 1);
@@ -663,6 +683,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
         const int steps = (len_max + kTileKeys - 1) / kTileKeys;
         if (warp < 4) {
             // ---------------- softmax: one row a thread
+            asm volatile("bar.sync 1, 128;" ::: "memory");                // no warp is a tile ahead of another
             const int row = tile * kTileRows + tid, tok = row / p.group, head = h * p.group + row - tok * p.group;
             const bool on = row < rows;
             const int len = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : len_max;
@@ -696,35 +717,32 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             float m = kNegInf, top = kNegInf, l = 0.f;
             for (int i = 0; i < steps; ++i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
-                prompt_wait(sh, &sh.full[stage], at / kPromptStages);      // the scales are there
-                prompt_wait(sh, &sh.s_full[at & 1], at >> 1);
+                warp_wait(sh, &sh.full[stage], at / kPromptStages);      // the scales are there
+                warp_wait(sh, &sh.s_full[at & 1], at >> 1);
                 tc_fence_after();
-                // 32 scores at a time, read twice: all 64 of them and their weights do not fit the registers
-                float s[32];
-                auto half = [&](int d) {
-                    tmem_ld32(lanes + (at & 1) * kTileKeys + 32 * d, s);
-                    tmem_ld_wait();
-                    const int left = len - i * kTileKeys - 32 * d;         // scores from here on are masked
-                    if (i * kTileKeys + kTileKeys > len_min) {
+                float s[kTileKeys];
+                tmem_ld32(lanes + (at & 1) * kTileKeys, s);
+                tmem_ld32(lanes + (at & 1) * kTileKeys + 32, s + 32);
+                tmem_ld_wait();
+                if (i * kTileKeys + kTileKeys > len_min) {
+                    const int left = len - i * kTileKeys;                  // scores from here on are masked
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (k >= left) s[k] = kNegInf;
-                    }
-                };
+                    for (int k = 0; k < kTileKeys; ++k)
+                        if (k >= left) s[k] = kNegInf;
+                }
                 float ck[4], m1 = m, t1 = top;
 #pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    half(d);
+                for (int u = 0; u < 4; ++u) {
+                    float mx[3];
 #pragma unroll
-                    for (int u = 2 * d; u < 2 * d + 2; ++u) {
-                        float mx = s[16 * (u & 1)];
+                    for (int k = 0; k < 3; ++k) mx[k] = max3(s[16 * u + 5 * k], s[16 * u + 5 * k + 1], s[16 * u + 5 * k + 2]);
 #pragma unroll
-                        for (int k = 1; k < 16; ++k) mx = fmaxf(mx, s[16 * (u & 1) + k]);
-                        ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);       // never 0: a masked score times it stays -inf
-                        mx = fmaf(mx, ck[u], sh.bias[stage][u]);
-                        m1 = fmaxf(m1, mx);
-                        t1 = fmaxf(t1, mx + sh.ev[stage][u]);
-                    }
+                    for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * u + 5 * k + 3], s[16 * u + 5 * k + 4]);
+                    mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * u + 15]);
+                    ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);           // never 0: a masked score times it stays -inf
+                    const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
+                    m1 = fmaxf(m1, x);
+                    t1 = fmaxf(t1, x + sh.ev[stage][u]);
                 }
                 const float mu = m1 == kNegInf ? 0.f : m1;
                 l *= ex2(m - mu);
@@ -735,31 +753,61 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                     top = t1;
                 }
                 const float tu = top == kNegInf ? 0.f : top;
-                if (i > 1) {                                               // this P has been read
-                    prompt_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
-                    tc_fence_after();
+                // weights straight as 2^(s + ev - top), their sum put back to 2^(s - m); a page whose V scale is so small that
+                // its weights vanish (a page of zeros) still counts in the sum: in two steps there
+                float ev[4], shift[4], lf[4];
+                bool plain = true;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    ev[u] = sh.ev[stage][u];
+                    lf[u] = mu + ev[u] - tu;
+                    shift[u] = sh.bias[stage][u] + ev[u] - tu;
+                    plain &= lf[u] > -60.f;
                 }
+                uint32_t pk[kTileKeys / 2];
+                if (__all_sync(kFullMask, plain)) {
+                    // in the order that hides the exponentials' latency: all arguments, all exponentials, then their uses
 #pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    half(d);
-                    uint32_t pk[16];
+                    for (int k = 0; k < kTileKeys; k += 2) {
+                        const float2 x = fma2(make_float2(s[k], s[k + 1]), make_float2(ck[k / 16], ck[k / 16]),
+                                              make_float2(shift[k / 16], shift[k / 16]));
+                        s[k] = x.x;
+                        s[k + 1] = x.y;
+                    }
 #pragma unroll
-                    for (int u = 2 * d; u < 2 * d + 2; ++u) {
-                        const float f = ex2(fminf(mu + sh.ev[stage][u] - tu, 127.f));
-                        const float shift = sh.bias[stage][u] - mu;
+                    for (int k = 0; k < kTileKeys; ++k) s[k] = ex2(s[k]);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        float2 sum = make_float2(s[16 * u], s[16 * u + 1]);
+                        pk[8 * u] = pack_f16x2(s[16 * u], s[16 * u + 1]);
+#pragma unroll
+                        for (int k = 2; k < 16; k += 2) {
+                            sum = add2(sum, make_float2(s[16 * u + k], s[16 * u + k + 1]));
+                            pk[8 * u + k / 2] = pack_f16x2(s[16 * u + k], s[16 * u + k + 1]);
+                        }
+                        l = fmaf(sum.x + sum.y, ex2(-lf[u]), l);
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float f = ex2(fminf(lf[u], 127.f)), to_m = shift[u] - lf[u];
                         float sum = 0.f;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            const float a = ex2(fmaf(s[16 * (u & 1) + k], ck[u], shift)), b = ex2(fmaf(s[16 * (u & 1) + k + 1], ck[u], shift));
+                            const float a = ex2(fmaf(s[16 * u + k], ck[u], to_m)), b = ex2(fmaf(s[16 * u + k + 1], ck[u], to_m));
                             sum += a + b;
-                            pk[8 * (u & 1) + k / 2] = pack_f16x2(a * f, b * f);
+                            pk[8 * u + k / 2] = pack_f16x2(a * f, b * f);
                         }
                         l += sum;
                     }
-                    tmem_st16(lanes + kColP + (at & 1) * 32 + 16 * d, pk);
                 }
+                if (i > 1) {                                               // this P has been read
+                    warp_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
+                    tc_fence_after();
+                }
+                tmem_st32(lanes + kColP + (at & 1) * 32, pk);
                 if (i > 0 && __any_sync(kFullMask, turn != 1.f)) {
-                    prompt_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
+                    warp_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
                     tc_fence_after();
 #pragma unroll
                     for (int d = 0; d < 2; ++d) {
@@ -772,11 +820,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&sh.p_full);
+                mbar_arrive(&sh.p_full[at & 1]);                           // two: a warp may be a step ahead of another
             }
             float f = 0.f;
             if (steps > 0) {
-                prompt_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1);
+                warp_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1);
                 tc_fence_after();
                 f = l == 0.f ? 0.f : ex2(top - m) / l;
             }
@@ -800,78 +848,70 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             if (on && p.lse) p.lse[(long long)(first + tok) * p.q_heads + head] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
             tc_fence_before();                                             // the accumulator is read: the next tile may write it
         } else if (warp < 6) {
-            // ---------------- e4m3 pages to f16 tiles: a thread carries 16 bytes of kRowsEach K rows and as many V rows
+            // ---------------- e4m3 pages to f16 tiles: a thread carries 16 bytes of one K row and of one V row of each unit of
+            // 16 keys; the pages of the next 32 units (8 steps) and their scales are held one a lane
             const int pid = tid - 128, key = pid >> 2, part = pid & 3;
-            constexpr int kApart = kProducers / 4;                         // rows between a thread's
-            const uint8_t* from = c.cache + (long long)h * c.head_stride + 16 * part;
-            const uint8_t* scales = c.scales + 2 * h;
-            uint4 kq[kRowsEach], vq[kRowsEach];
-            int page[kRowsEach], group_page = -1;                          // of the step after the one in kq, vq
-            uint32_t sc = 0;                                               // scales of 16 keys; 0xffffffff: no page
-            auto page_of = [&](int at) {
-                if (at >= len_max) return -1;
-                const int page = table[at >> c.page_shift];
-                return page < c.pages ? page : -1;
-            };
-            auto look_up = [&](int i) {
-#pragma unroll
-                for (int j = 0; j < kRowsEach; ++j) page[j] = page_of(i * kTileKeys + key + kApart * j);
-                if (pid < 4) group_page = page_of(i * kTileKeys + 16 * pid);
-            };
-            auto load = [&](int i) {
-#pragma unroll
-                for (int j = 0; j < kRowsEach; ++j) {
-                    const int at = i * kTileKeys + key + kApart * j;
-                    const bool live = page[j] >= 0 && at < len_max;
-                    const uint8_t* src = from + (long long)page[j] * c.page_stride +
-                                         (long long)(at & ((1 << c.page_shift) - 1)) * c.token_stride;
-                    kq[j] = live ? ld_stream_16(src + c.k_off) : make_uint4(0, 0, 0, 0);
-                    vq[j] = live ? ld_stream_16(src + c.v_off) : make_uint4(0, 0, 0, 0);
+            static_assert(kProducers == 64 && kTileKeys == 64, "16 rows of four parts: one unit");
+            const uint8_t* from = c.cache + (long long)h * c.head_stride + c.k_off + key * c.token_stride + 16 * part;
+            const long long v_from_k = c.v_off - c.k_off;
+            const int in_page = (1 << c.page_shift) - 1;
+            unsigned char* mine = raw_ring + pid * 16;                     // K parts, then V parts; read back by their writer
+            const uint32_t lo_at = key * 128 + ((2 * part) ^ (key & 7)) * 16, hi_at = key * 128 + ((2 * part + 1) ^ (key & 7)) * 16;
+            int pages = -1;
+            uint32_t scale2 = 0, used_scale2 = 0;                          // of the units being fetched, being converted
+            int used_pages = -1;
+            auto fetch = [&](int i) {
+                if ((i & 7) == 0) {
+                    const int unit = 4 * i + lane;
+                    used_pages = pages;
+                    used_scale2 = scale2;
+                    pages = unit * 16 < len_max ? table[unit * 16 >> c.page_shift] : -1;
+                    if (pages >= c.pages || pages < 0) pages = -1;
+                    scale2 = pages < 0 ? 0u : *reinterpret_cast<const uint16_t*>(c.scales + ((long long)pages * c.kv_heads + h) * 2);
                 }
-                if (pid < 4)
-                    sc = group_page < 0 ? 0xffffffffu
-                                        : *reinterpret_cast<const uint16_t*>(scales + (long long)group_page * c.kv_heads * 2);
+                unsigned char* to = mine + (i % kRawStages) * kRawBytes;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int page = __shfl_sync(kFullMask, pages, (4 * i + u) & 31), at = i * kTileKeys + 16 * u;
+                    const bool live = page >= 0 && at + key < len_max;
+                    const uint8_t* src = from + (live ? (long long)page * c.page_stride + (long long)(at & in_page) * c.token_stride : 0);
+                    cp_async16(to + u * kProducers * 16, src, live);
+                    cp_async16(to + (4 + u) * kProducers * 16, src + v_from_k, live);
+                }
+                cp_async_commit();
             };
-            look_up(0);
-            load(0);
-            look_up(1);
+            for (int i = 0; i < kRawStages - 1; ++i) fetch(i);
             for (int i = 0; i < steps; ++i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
-                if (at >= kPromptStages) prompt_wait(sh, &sh.empty[stage], at / kPromptStages - 1);
+                fetch(i + kRawStages - 1);                                 // steps past the last fetch zeros
+                cp_async_wait<kRawStages - 1>();
+                if (at >= kPromptStages) warp_wait(sh, &sh.empty[stage], at / kPromptStages - 1);
                 unsigned char* k_tile = kv_tiles + stage * 2 * kTileKeys * 128;
+                const unsigned char* raw16 = mine + (i % kRawStages) * kRawBytes;
 #pragma unroll
-                for (int j = 0; j < kRowsEach; ++j) {
-                    const int row = key + kApart * j;
-                    unsigned char* to = k_tile + row * 128;
-                    const uint32_t a = ((2 * part) ^ (row & 7)) * 16, b = ((2 * part + 1) ^ (row & 7)) * 16;
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(raw16 + j * kProducers * 16);
+                    unsigned char* to = k_tile + j * 16 * 128;             // four units of K, then of V
                     uint4 lo, hi;
-                    e4m3x4_to_f16(kq[j].x, lo.x, lo.y);
-                    e4m3x4_to_f16(kq[j].y, lo.z, lo.w);
-                    e4m3x4_to_f16(kq[j].z, hi.x, hi.y);
-                    e4m3x4_to_f16(kq[j].w, hi.z, hi.w);
-                    *reinterpret_cast<uint4*>(to + a) = lo;
-                    *reinterpret_cast<uint4*>(to + b) = hi;
-                    e4m3x4_to_f16(vq[j].x, lo.x, lo.y);
-                    e4m3x4_to_f16(vq[j].y, lo.z, lo.w);
-                    e4m3x4_to_f16(vq[j].z, hi.x, hi.y);
-                    e4m3x4_to_f16(vq[j].w, hi.z, hi.w);
-                    *reinterpret_cast<uint4*>(to + kTileKeys * 128 + a) = lo;
-                    *reinterpret_cast<uint4*>(to + kTileKeys * 128 + b) = hi;
+                    e4m3x4_to_f16(v.x, lo.x, lo.y);
+                    e4m3x4_to_f16(v.y, lo.z, lo.w);
+                    e4m3x4_to_f16(v.z, hi.x, hi.y);
+                    e4m3x4_to_f16(v.w, hi.z, hi.w);
+                    *reinterpret_cast<uint4*>(to + lo_at) = lo;
+                    *reinterpret_cast<uint4*>(to + hi_at) = hi;
                 }
-                const uint32_t scale2 = sc;
-                if (i + 1 < steps) {
-                    load(i + 1);
-                    look_up(i + 2);
-                }
-                if (pid < 4) {
-                    const bool none = scale2 == 0xffffffffu;
-                    sh.ks[stage][pid] = none ? 0.f : exp2_biased(scale2 & 0xffu);
-                    sh.ev[stage][pid] = none ? 0.f : (float)(int)(scale2 >> 8) - 127.f;
-                    sh.bias[stage][pid] = none ? kNegInf : 0.f;
+                const bool older = ((i + kRawStages - 1) & ~7) != (i & ~7);
+                if (warp == 4 && (lane >> 2) == (i & 7)) {
+                    const bool none = (older ? used_pages : pages) < 0;
+                    const uint32_t two = older ? used_scale2 : scale2;
+                    sh.ks[stage][lane & 3] = exp2_biased(two & 0xffu);
+                    sh.ev[stage][lane & 3] = (float)(int)(two >> 8) - 127.f;
+                    sh.bias[stage][lane & 3] = none ? kNegInf : 0.f;
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.full[stage]);
             }
+            cp_async_wait<0>();                                            // the next tile's copies go to the same places
         } else if (warp == 6 && lane == 0) {
             // ---------------- products
             prompt_wait(sh, &sh.q_full, tiles_done);
@@ -890,7 +930,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             for (int i = 0; i < steps; ++i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
                 if (i + 1 < steps) scores(i + 1);
-                prompt_wait(sh, &sh.p_full, at);
+                prompt_wait(sh, &sh.p_full[at & 1], at >> 1);
                 tc_fence_after();
                 const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
 #pragma unroll
