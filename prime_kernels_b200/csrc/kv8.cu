@@ -615,7 +615,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {
         : "r"(at)
         : "memory");
 }
-template <typename T> __device__ __forceinline__ void tmem_st32(uint32_t at, const T* v) {
+__device__ __forceinline__ void tmem_st32(uint32_t at, const float* v) {
     const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -624,6 +624,13 @@ template <typename T> __device__ __forceinline__ void tmem_st32(uint32_t at, con
         "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
         "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
         "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(at)
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -720,29 +727,37 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 warp_wait(sh, &sh.full[stage], at / kPromptStages);      // the scales are there
                 warp_wait(sh, &sh.s_full[at & 1], at >> 1);
                 tc_fence_after();
-                float s[kTileKeys];
-                tmem_ld32(lanes + (at & 1) * kTileKeys, s);
-                tmem_ld32(lanes + (at & 1) * kTileKeys + 32, s + 32);
-                tmem_ld_wait();
-                if (i * kTileKeys + kTileKeys > len_min) {
-                    const int left = len - i * kTileKeys;                  // scores from here on are masked
+                // 32 scores at a time, the first 32 read twice: 64 and their weights do not fit the registers, and a spill
+                // costs an L2 access here (shared memory leaves next to no L1)
+                float s[32];
+                auto read = [&](int d) {
+                    tmem_ld32(lanes + (at & 1) * kTileKeys + 32 * d, s);
+                    tmem_ld_wait();
+                    if (i * kTileKeys + kTileKeys > len_min) {
+                        const int left = len - i * kTileKeys - 32 * d;     // scores from here on are masked
 #pragma unroll
-                    for (int k = 0; k < kTileKeys; ++k)
-                        if (k >= left) s[k] = kNegInf;
-                }
+                        for (int k = 0; k < 32; ++k)
+                            if (k >= left) s[k] = kNegInf;
+                    }
+                };
                 float ck[4], m1 = m, t1 = top;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float mx[3];
+                for (int d = 0; d < 2; ++d) {
+                    read(d);
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) mx[k] = max3(s[16 * u + 5 * k], s[16 * u + 5 * k + 1], s[16 * u + 5 * k + 2]);
+                    for (int v = 0; v < 2; ++v) {
+                        const int u = 2 * d + v;
+                        float mx[3];
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * u + 5 * k + 3], s[16 * u + 5 * k + 4]);
-                    mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * u + 15]);
-                    ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);           // never 0: a masked score times it stays -inf
-                    const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
-                    m1 = fmaxf(m1, x);
-                    t1 = fmaxf(t1, x + sh.ev[stage][u]);
+                        for (int k = 0; k < 3; ++k) mx[k] = max3(s[16 * v + 5 * k], s[16 * v + 5 * k + 1], s[16 * v + 5 * k + 2]);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * v + 5 * k + 3], s[16 * v + 5 * k + 4]);
+                        mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * v + 15]);
+                        ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);       // never 0: a masked score times it stays -inf
+                        const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
+                        m1 = fmaxf(m1, x);
+                        t1 = fmaxf(t1, x + sh.ev[stage][u]);
+                    }
                 }
                 const float mu = m1 == kNegInf ? 0.f : m1;
                 l *= ex2(m - mu);
@@ -755,57 +770,59 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 const float tu = top == kNegInf ? 0.f : top;
                 // weights straight as 2^(s + ev - top), their sum put back to 2^(s - m); a page whose V scale is so small that
                 // its weights vanish (a page of zeros) still counts in the sum: in two steps there
-                float ev[4], shift[4], lf[4];
-                bool plain = true;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    ev[u] = sh.ev[stage][u];
-                    lf[u] = mu + ev[u] - tu;
-                    shift[u] = sh.bias[stage][u] + ev[u] - tu;
-                    plain &= lf[u] > -60.f;
-                }
-                uint32_t pk[kTileKeys / 2];
-                if (__all_sync(kFullMask, plain)) {
-                    // in the order that hides the exponentials' latency: all arguments, all exponentials, then their uses
-#pragma unroll
-                    for (int k = 0; k < kTileKeys; k += 2) {
-                        const float2 x = fma2(make_float2(s[k], s[k + 1]), make_float2(ck[k / 16], ck[k / 16]),
-                                              make_float2(shift[k / 16], shift[k / 16]));
-                        s[k] = x.x;
-                        s[k + 1] = x.y;
-                    }
-#pragma unroll
-                    for (int k = 0; k < kTileKeys; ++k) s[k] = ex2(s[k]);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        float2 sum = make_float2(s[16 * u], s[16 * u + 1]);
-                        pk[8 * u] = pack_f16x2(s[16 * u], s[16 * u + 1]);
-#pragma unroll
-                        for (int k = 2; k < 16; k += 2) {
-                            sum = add2(sum, make_float2(s[16 * u + k], s[16 * u + k + 1]));
-                            pk[8 * u + k / 2] = pack_f16x2(s[16 * u + k], s[16 * u + k + 1]);
-                        }
-                        l = fmaf(sum.x + sum.y, ex2(-lf[u]), l);
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const float f = ex2(fminf(lf[u], 127.f)), to_m = shift[u] - lf[u];
-                        float sum = 0.f;
-#pragma unroll
-                        for (int k = 0; k < 16; k += 2) {
-                            const float a = ex2(fmaf(s[16 * u + k], ck[u], to_m)), b = ex2(fmaf(s[16 * u + k + 1], ck[u], to_m));
-                            sum += a + b;
-                            pk[8 * u + k / 2] = pack_f16x2(a * f, b * f);
-                        }
-                        l += sum;
-                    }
-                }
                 if (i > 1) {                                               // this P has been read
                     warp_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
                     tc_fence_after();
                 }
-                tmem_st32(lanes + kColP + (at & 1) * 32, pk);
+#pragma unroll
+                for (int d = 1; d >= 0; --d) {
+                    if (d == 0) read(0);
+                    float shift[2], lf[2];
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const float ev = sh.ev[stage][2 * d + v];
+                        lf[v] = mu + ev - tu;
+                        shift[v] = sh.bias[stage][2 * d + v] + ev - tu;
+                    }
+                    uint32_t pk[16];
+                    if (__all_sync(kFullMask, fminf(lf[0], lf[1]) > -60.f)) {
+                        // in the order that hides the exponentials' latency: all arguments, all exponentials, then their uses
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const float2 x = fma2(make_float2(s[k], s[k + 1]), make_float2(ck[2 * d + k / 16], ck[2 * d + k / 16]),
+                                                  make_float2(shift[k / 16], shift[k / 16]));
+                            s[k] = x.x;
+                            s[k + 1] = x.y;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[k] = ex2(s[k]);
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            float2 sum = make_float2(s[16 * v], s[16 * v + 1]);
+                            pk[8 * v] = pack_f16x2(s[16 * v], s[16 * v + 1]);
+#pragma unroll
+                            for (int k = 2; k < 16; k += 2) {
+                                sum = add2(sum, make_float2(s[16 * v + k], s[16 * v + k + 1]));
+                                pk[8 * v + k / 2] = pack_f16x2(s[16 * v + k], s[16 * v + k + 1]);
+                            }
+                            l = fmaf(sum.x + sum.y, ex2(-lf[v]), l);
+                        }
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            const float f = ex2(fminf(lf[v], 127.f)), to_m = sh.bias[stage][2 * d + v] - mu;
+                            float sum = 0.f;
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) {
+                                const float a = ex2(fmaf(s[16 * v + k], ck[2 * d + v], to_m)), b = ex2(fmaf(s[16 * v + k + 1], ck[2 * d + v], to_m));
+                                sum += a + b;
+                                pk[8 * v + k / 2] = pack_f16x2(a * f, b * f);
+                            }
+                            l += sum;
+                        }
+                    }
+                    tmem_st16(lanes + kColP + (at & 1) * 32 + 16 * d, pk);
+                }
                 if (i > 0 && __any_sync(kFullMask, turn != 1.f)) {
                     warp_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
                     tc_fence_after();
