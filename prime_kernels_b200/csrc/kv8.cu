@@ -551,10 +551,6 @@ constexpr int kRawStages = 4, kRawBytes = kTileKeys * 128;              // e4m3 
 constexpr int kPromptThreads = 256, kProducers = 64;
 constexpr uint32_t kPromptCols = 256, kColP = 128, kColO = 192;            // S in columns 0..127, P in 128..191, two of each
 constexpr float kLazy = 8.f;
-#ifndef PK_MINROWS
-#define PK_MINROWS 64
-#endif
-constexpr int kPromptMinRows = PK_MINROWS;
 
 struct PromptShared {
     uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full[2], pv_done[2], drain;
@@ -663,8 +659,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             mbar_init(&sh.empty[i], 1);
         }
         mbar_init(&sh.q_full, 128);
-        mbar_init(&sh.s_full[0], 1);
-        mbar_init(&sh.s_full[1], 1);
+        mbar_init(&sh.s_full[0], 2);                                       // the products, and the thread that saw the scales
+        mbar_init(&sh.s_full[1], 2);
         mbar_init(&sh.p_full[0], 128);
         mbar_init(&sh.p_full[1], 128);
         mbar_init(&sh.pv_done[0], 1);
@@ -691,11 +687,12 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
         if (warp < 4) {
             // ---------------- softmax: one row a thread
             asm volatile("bar.sync 1, 128;" ::: "memory");                // no warp is a tile ahead of another
-            const int row = tile * kTileRows + tid, tok = row / p.group, head = h * p.group + row - tok * p.group;
-            const bool on = row < rows;
-            const int len = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : len_max;
             float qs;
+            int len;
             {
+                const int row = tile * kTileRows + tid, tok = row / p.group, head = h * p.group + row - tok * p.group;
+                const bool on = row < rows;
+                len = on ? (int)min((long long)max(seq - count + tok + 1, 0), capacity) : len_max;
                 uint4 w[8];
                 const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(first + tok) * p.q_token + (long long)head * p.q_head);
                 float amax = 0.f;
@@ -724,40 +721,31 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             float m = kNegInf, top = kNegInf, l = 0.f;
             for (int i = 0; i < steps; ++i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
-                warp_wait(sh, &sh.full[stage], at / kPromptStages);      // the scales are there
                 warp_wait(sh, &sh.s_full[at & 1], at >> 1);
                 tc_fence_after();
-                // 32 scores at a time, the first 32 read twice: 64 and their weights do not fit the registers, and a spill
-                // costs an L2 access here (shared memory leaves next to no L1)
-                float s[32];
-                auto read = [&](int d) {
-                    tmem_ld32(lanes + (at & 1) * kTileKeys + 32 * d, s);
-                    tmem_ld_wait();
-                    if (i * kTileKeys + kTileKeys > len_min) {
-                        const int left = len - i * kTileKeys - 32 * d;     // scores from here on are masked
+                float s[kTileKeys];
+                tmem_ld32(lanes + (at & 1) * kTileKeys, s);
+                tmem_ld32(lanes + (at & 1) * kTileKeys + 32, s + 32);
+                tmem_ld_wait();
+                if (i * kTileKeys + kTileKeys > len_min) {
+                    const int left = len - i * kTileKeys;                  // scores from here on are masked
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (k >= left) s[k] = kNegInf;
-                    }
-                };
+                    for (int k = 0; k < kTileKeys; ++k)
+                        if (k >= left) s[k] = kNegInf;
+                }
                 float ck[4], m1 = m, t1 = top;
 #pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    read(d);
+                for (int u = 0; u < 4; ++u) {
+                    float mx[3];
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const int u = 2 * d + v;
-                        float mx[3];
+                    for (int k = 0; k < 3; ++k) mx[k] = max3(s[16 * u + 5 * k], s[16 * u + 5 * k + 1], s[16 * u + 5 * k + 2]);
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) mx[k] = max3(s[16 * v + 5 * k], s[16 * v + 5 * k + 1], s[16 * v + 5 * k + 2]);
-#pragma unroll
-                        for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * v + 5 * k + 3], s[16 * v + 5 * k + 4]);
-                        mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * v + 15]);
-                        ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);       // never 0: a masked score times it stays -inf
-                        const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
-                        m1 = fmaxf(m1, x);
-                        t1 = fmaxf(t1, x + sh.ev[stage][u]);
-                    }
+                    for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * u + 5 * k + 3], s[16 * u + 5 * k + 4]);
+                    mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * u + 15]);
+                    ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);           // never 0: a masked score times it stays -inf
+                    const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
+                    m1 = fmaxf(m1, x);
+                    t1 = fmaxf(t1, x + sh.ev[stage][u]);
                 }
                 const float mu = m1 == kNegInf ? 0.f : m1;
                 l *= ex2(m - mu);
@@ -775,8 +763,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                     tc_fence_after();
                 }
 #pragma unroll
-                for (int d = 1; d >= 0; --d) {
-                    if (d == 0) read(0);
+                for (int d = 0; d < 2; ++d) {
                     float shift[2], lf[2];
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
@@ -789,21 +776,21 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                         // in the order that hides the exponentials' latency: all arguments, all exponentials, then their uses
 #pragma unroll
                         for (int k = 0; k < 32; k += 2) {
-                            const float2 x = fma2(make_float2(s[k], s[k + 1]), make_float2(ck[2 * d + k / 16], ck[2 * d + k / 16]),
+                            const float2 x = fma2(make_float2(s[32 * d + k], s[32 * d + k + 1]), make_float2(ck[2 * d + k / 16], ck[2 * d + k / 16]),
                                                   make_float2(shift[k / 16], shift[k / 16]));
-                            s[k] = x.x;
-                            s[k + 1] = x.y;
+                            s[32 * d + k] = x.x;
+                            s[32 * d + k + 1] = x.y;
                         }
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) s[k] = ex2(s[k]);
+                        for (int k = 0; k < 32; ++k) s[32 * d + k] = ex2(s[32 * d + k]);
 #pragma unroll
                         for (int v = 0; v < 2; ++v) {
-                            float2 sum = make_float2(s[16 * v], s[16 * v + 1]);
-                            pk[8 * v] = pack_f16x2(s[16 * v], s[16 * v + 1]);
+                            float2 sum = make_float2(s[32 * d + 16 * v], s[32 * d + 16 * v + 1]);
+                            pk[8 * v] = pack_f16x2(s[32 * d + 16 * v], s[32 * d + 16 * v + 1]);
 #pragma unroll
                             for (int k = 2; k < 16; k += 2) {
-                                sum = add2(sum, make_float2(s[16 * v + k], s[16 * v + k + 1]));
-                                pk[8 * v + k / 2] = pack_f16x2(s[16 * v + k], s[16 * v + k + 1]);
+                                sum = add2(sum, make_float2(s[32 * d + 16 * v + k], s[32 * d + 16 * v + k + 1]));
+                                pk[8 * v + k / 2] = pack_f16x2(s[32 * d + 16 * v + k], s[32 * d + 16 * v + k + 1]);
                             }
                             l = fmaf(sum.x + sum.y, ex2(-lf[v]), l);
                         }
@@ -814,7 +801,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                             float sum = 0.f;
 #pragma unroll
                             for (int k = 0; k < 16; k += 2) {
-                                const float a = ex2(fmaf(s[16 * v + k], ck[2 * d + v], to_m)), b = ex2(fmaf(s[16 * v + k + 1], ck[2 * d + v], to_m));
+                                const float a = ex2(fmaf(s[32 * d + 16 * v + k], ck[2 * d + v], to_m)), b = ex2(fmaf(s[32 * d + 16 * v + k + 1], ck[2 * d + v], to_m));
                                 sum += a + b;
                                 pk[8 * v + k / 2] = pack_f16x2(a * f, b * f);
                             }
@@ -845,6 +832,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 tc_fence_after();
                 f = l == 0.f ? 0.f : ex2(top - m) / l;
             }
+            int again = tid;                                               // worked out once more: not kept in registers over the loop
+            asm volatile("" : "+r"(again));
+            const int row = tile * kTileRows + again, tok = row / p.group, head = h * p.group + row - tok * p.group;
+            const bool on = row < rows;
             uint4* to = reinterpret_cast<uint4*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head);
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
@@ -942,6 +933,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 for (int k = 0; k < 4; ++k)                                // 16 dims = 32 bytes a product
                     mma_ss(tmem + (at & 1) * kTileKeys, dq + 2 * k, dk + 2 * k, kIdescQK, k > 0);
                 mma_commit(&sh.s_full[at & 1]);
+                mbar_arrive(&sh.s_full[at & 1]);                           // hands on the scales that came with the tile
             };
             if (steps > 0) scores(0);
             for (int i = 0; i < steps; ++i) {
@@ -1055,7 +1047,13 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     if ((long long)longest * p.group > 0x7fffffffLL - 16) return kErrShape;
     // rows a request is expected to have: the longest where the caller knows it, else the mean
     const long long expected = (max_query_len > 0 || !p.c.cu ? (long long)longest : ((long long)tokens + p.c.batch - 1) / p.c.batch) * p.group;
-    if (expected >= kPromptMinRows) {
+    // The prompt kernel's tile of 128 rows takes 1.2 us for 64 keys however few of them there are, and no tile's keys are
+    // split; the other kernel's rate does not depend on either.  They meet at 740 tiles of 16 rows where the SMs are not
+    // full, and at tiles of 128 rows that are 45 % full: 1 request of 128 tokens, 15/5 heads (120 tiles) 77 us against
+    // 23; 8 of 32, 32/32 heads (512) 45 against 29; 16 of 256, 9/3 heads (2304) 85 against 131; 32 of 64, 32/32 heads
+    // (4096, half full) 77 against 108.
+    const long long sets = (long long)p.c.kv_heads * p.c.batch, small = (expected + 15) / 16 * sets;
+    if (small >= 740 && 10 * small >= 36 * ((expected + kTileRows - 1) / kTileRows) * sets) {
         const long long tiles = ((long long)longest * p.group + kTileRows - 1) / kTileRows;
         p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
         const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptBytes);

@@ -102,23 +102,22 @@ def attend64(q, held, table, seq, cu, scale):
         k, v, ok = held.values(pages)
         k, v, ok = k[:length], v[:length], ok[:length]
         top = np.array([2.0 ** float(held.e[p].max() - 127) for p in pages if 0 <= p < len(held.x)] or [0.0]).max()
-        for j in range(n):
-            upto = min(max(int(seq[r]) - n + j + 1, 0), length)
-            live = np.nonzero(ok[:upto])[0]
-            if not len(live):
-                continue
-            for h in range(heads):
-                kk, vv = k[live, h // group], v[live, h // group]
-                s = kk @ q[a + j, h] * scale
-                ds = 2.0 ** -15 * (np.abs(kk) @ np.abs(q[a + j, h])).max() * abs(scale)
-                m = s.max()
-                w = np.exp(s - m)
-                z = w.sum()
-                out[a + j, h], lse[a + j, h] = w @ vv / z, m + math.log(z)
-                spread = w @ np.abs(vv) / z
-                tol[a + j, h] = (2.0 ** -8 * np.abs(out[a + j, h]) + spread * (2.0 ** -11 + 2.0 ** -18 + 2 * ds) +
-                                 len(live) * 2.0 ** -25 * 448 * top / z)
-                tol_lse[a + j, h] = ds + 2.0 ** -21 * (1 + abs(m) + math.log(z))
+        upto = np.clip(int(seq[r]) - n + 1 + np.arange(n), 0, length)
+        sees = (np.arange(length) < upto[:, None]) & ok                                    # [n, length]
+        some = sees.any(1)
+        for h in range(heads):
+            kk, vv, qq = k[:, h // group], v[:, h // group], q[a:b, h]
+            s = np.where(sees, qq @ kk.T * scale, -np.inf)
+            ds = 2.0 ** -15 * np.where(sees, np.abs(qq) @ np.abs(kk).T, 0.0).max(1, initial=0.0) * abs(scale)
+            m = np.where(some, s.max(1, initial=-np.inf), 0.0)
+            w = np.exp(s - m[:, None])
+            z = np.where(some, w.sum(1), 1.0)
+            out[a:b, h] = w @ vv / z[:, None]
+            lse[a:b, h] = np.where(some, m + np.log(z), -np.inf)
+            spread = w @ np.abs(vv) / z[:, None]
+            tol[a:b, h] = (2.0 ** -8 * np.abs(out[a:b, h]) + spread * (2.0 ** -11 + 2.0 ** -18 + 2 * ds)[:, None] +
+                           (sees.sum(1) * 2.0 ** -25 * 448 * top / z)[:, None])
+            tol_lse[a:b, h] = ds + 2.0 ** -21 * (1 + np.abs(m) + np.log(z))
     return out, lse, tol, tol_lse, mine
 
 
@@ -282,7 +281,7 @@ def test_decode_attention_spread_over_ctas(cuda_device, batch, length):
 
 
 @pytest.mark.parametrize("heads,group", [(1, 1), (3, 3), (2, 5)])
-@pytest.mark.parametrize("new", [[2, 5, 0, 1, 9], [33, 16, 0, 130, 7], [1, 1, 300, 64, 65]])
+@pytest.mark.parametrize("new", [[2, 5, 0, 1, 9], [33, 16, 0, 130, 7], [1, 1, 300, 64, 65], [700, 3, 0, 260, 515], [128, 64, 0, 1200, 641]])
 @pytest.mark.parametrize("known", [True, False])
 def test_ragged_queries(cuda_device, heads, group, new, known):
     """Several query tokens each, causal among themselves; rows behind the last request are left alone."""
@@ -290,7 +289,7 @@ def test_ragged_queries(cuda_device, heads, group, new, known):
     seq = [new[0], new[1] + 40, 9, new[3] + 333, new[4] + 16]
     cache, scales, table, lens = filled(g, seq, heads, 16, heads == 2, cuda_device)
     cu = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32)
-    q = torch.randn(sum(new) + 6, heads * group, D, generator=g).bfloat16()
+    q = torch.randn(sum(new) + 6, heads * group + 2, D, generator=g).bfloat16()[:, 1:-1]
     out = torch.full(q.shape, 77.0, dtype=torch.bfloat16, device=cuda_device)
     run_attention(cuda_device, cache, scales, table, lens, q, cu, max_query_len=max(new) if known else None, out=out)
     assert (out[sum(new):] == 77).all()
@@ -298,18 +297,20 @@ def test_ragged_queries(cuda_device, heads, group, new, known):
     run_attention(cuda_device, cache, scales, table, lens, q, cu, max_query_len=1)
 
 
-def test_more_queries_than_positions(cuda_device):
+@pytest.mark.parametrize("heads,group,first,second", [(2, 2, 12, 8), (4, 4, 700, 600)])
+def test_more_queries_than_positions(cuda_device, heads, group, first, second):
     """Rows before position 0 see nothing: zeros and -inf."""
     g = torch.Generator().manual_seed(3)
-    cache, scales, table, lens = filled(g, [5, 40], 2, 16, False, cuda_device)
-    cu = torch.tensor([0, 12, 20], dtype=torch.int32)
-    q = torch.randn(20, 4, D, generator=g).bfloat16()
+    cache, scales, table, lens = filled(g, [5, 40], heads, 16, False, cuda_device)
+    cu = torch.tensor([0, first, first + second], dtype=torch.int32)
+    q = torch.randn(first + second, heads * group, D, generator=g).bfloat16()
     out, lse = run_attention(cuda_device, cache, scales, table, lens, q, cu)
-    assert (out[:7] == 0).all() and (lse[:7] == -math.inf).all()
+    assert (out[: first - 5] == 0).all() and (lse[: first - 5] == -math.inf).all()
+    run_attention(cuda_device, cache, scales, table, lens, q, cu, max_query_len=max(first, second))
 
 
-@pytest.mark.parametrize("n", [1, 40])
-def test_scales_that_differ_from_page_to_page(cuda_device, n):
+@pytest.mark.parametrize("n,heads", [(1, 2), (40, 2), (333, 12)])
+def test_scales_that_differ_from_page_to_page(cuda_device, n, heads):
     """V scales over 60 binades, pages of zeros, large scores: no page's scale may hurt another's tokens."""
     g = torch.Generator().manual_seed(4)
 
@@ -320,14 +321,14 @@ def test_scales_that_differ_from_page_to_page(cuda_device, n):
         k = k * torch.exp2((i % 4 - 2).float())[:, None, None]
         return k, v
 
-    cache, scales, table, lens = filled(g, [400, 333], 2, 16, False, cuda_device, gain)
+    cache, scales, table, lens = filled(g, [400, 333], heads, 16, False, cuda_device, gain)
     cu = None if n == 1 else torch.tensor([0, n, 2 * n], dtype=torch.int32)
-    q = (4 * torch.randn(2 * n, 4, D, generator=g)).bfloat16()
+    q = (4 * torch.randn(2 * n, 2 * heads, D, generator=g)).bfloat16()
     run_attention(cuda_device, cache, scales, table, lens, q, cu)
 
 
-@pytest.mark.parametrize("n", [1, 40])
-def test_low_scale_pages_under_a_masked_high_scale_one(cuda_device, n):
+@pytest.mark.parametrize("n,heads,group", [(1, 1, 2), (40, 1, 2), (100, 12, 10)])
+def test_low_scale_pages_under_a_masked_high_scale_one(cuda_device, n, heads, group):
     """All the weight lies on pages whose V scale is 2^-30 of another page's that gets next to none of it."""
     from prime_kernels_b200 import kv8
 
@@ -339,8 +340,8 @@ def test_low_scale_pages_under_a_masked_high_scale_one(cuda_device, n):
         k[16:] = k[16:].abs()
         return k, v
 
-    cache, scales, table, lens = filled(g, [100], 1, 16, False, cuda_device, gain)
-    q = torch.rand(n, 2, D, generator=g).add(4.0).bfloat16()
+    cache, scales, table, lens = filled(g, [100 + n - 1], heads, 16, False, cuda_device, gain)
+    q = torch.rand(n, heads * group, D, generator=g).add(4.0).bfloat16()
     cu = None if n == 1 else torch.tensor([0, n], dtype=torch.int32)
     out = kv8.attention(q.to(cuda_device), cache, scales, table.to(cuda_device), lens.to(cuda_device),
                         None if cu is None else cu.to(cuda_device))
@@ -351,38 +352,54 @@ def test_low_scale_pages_under_a_masked_high_scale_one(cuda_device, n):
     assert (np.abs(out.double().cpu().numpy() - want) <= np.minimum(tol, tight)).all()
 
 
-@pytest.mark.parametrize("size", [1e-30, 1.0, 1e30])
-def test_q_of_any_size(cuda_device, size):
-    """q is brought into f16's range by a power of two per row; a row of zeros weighs all keys alike."""
+@pytest.mark.parametrize("n,heads", [(1, 1), (400, 10)])
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e30, -1.0, 0.0])
+def test_q_of_any_size(cuda_device, size, n, heads):
+    """q is brought into f16's range by a power of two per row; a row of zeros weighs all keys alike, and so does a scale
+    of 0; a negative scale turns the order round."""
     g = torch.Generator().manual_seed(6)
-    cache, scales, table, lens = filled(g, [77, 50], 1, 16, False, cuda_device)
-    q = torch.randn(2, 3, D, generator=g)
+    cache, scales, table, lens = filled(g, [76 + n, 449 + n], heads, 16, False, cuda_device)
+    q = torch.randn(2 * n, 3 * heads, D, generator=g)
     q[0, 1] = 0.0
-    run_attention(cuda_device, cache, scales, table, lens, (q * size).bfloat16(), scale=0.125 / size)
+    cu = None if n == 1 else torch.tensor([0, n, 2 * n], dtype=torch.int32)
+    run_attention(cuda_device, cache, scales, table, lens, (q * (abs(size) or 1.0)).bfloat16(), cu, scale=0.125 / size if size else 0.0)
 
 
-def test_pages_outside_the_pool_are_masked(cuda_device):
+@pytest.mark.parametrize("n,heads", [(1, 2), (16, 2), (300, 10)])
+def test_pages_outside_the_pool_are_masked(cuda_device, n, heads):
     g = torch.Generator().manual_seed(7)
-    cache, scales, table, lens = filled(g, [90, 64, 16], 2, 16, False, cuda_device)
+    cache, scales, table, lens = filled(g, [390, 368, 16], heads, 16, False, cuda_device)
     table[0, 2], table[1, 0], table[2, 0] = -1, 10 ** 6, -5          # the last request has nothing left
-    q = torch.randn(3, 6, D, generator=g).bfloat16()
-    out, lse = run_attention(cuda_device, cache, scales, table, lens, q)
-    assert (out[2] == 0).all() and (lse[2] == -math.inf).all()
+    q = torch.randn(3 * n, 3 * heads, D, generator=g).bfloat16()
+    cu = None if n == 1 else torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32)
+    out, lse = run_attention(cuda_device, cache, scales, table, lens, q, cu)
+    assert (out[2 * n:] == 0).all() and (lse[2 * n:] == -math.inf).all()
     lens[1] = 10 ** 6                                                # longer than its table: clamped to it
-    run_attention(cuda_device, cache, scales, table, lens, q)
+    run_attention(cuda_device, cache, scales, table, lens, q, cu)
     lens[0] = -4
-    run_attention(cuda_device, cache, scales, table, lens, q)
+    run_attention(cuda_device, cache, scales, table, lens, q, cu)
 
 
-def test_nan_is_not_hidden(cuda_device):
+@pytest.mark.parametrize("n,heads", [(1, 1), (400, 10)])
+def test_nan_is_not_hidden(cuda_device, n, heads):
     from prime_kernels_b200 import kv8
 
     g = torch.Generator().manual_seed(9)
-    cache, scales, table, lens = filled(g, [30, 30], 1, 16, False, cuda_device)
-    q = torch.randn(2, 1, D, generator=g).bfloat16()
+    cache, scales, table, lens = filled(g, [400, 410], heads, 16, False, cuda_device)
+    q = torch.randn(2 * n, 3 * heads, D, generator=g).bfloat16()
     q[0, 0, 5] = math.nan
-    out = kv8.attention(q.to(cuda_device), cache, scales, table.to(cuda_device), lens.to(cuda_device))
-    assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all()
+    cu = None if n == 1 else torch.tensor([0, n, 2 * n], dtype=torch.int32, device=cuda_device)
+    out = kv8.attention(q.to(cuda_device), cache, scales, table.to(cuda_device), lens.to(cuda_device), cu)
+    assert torch.isnan(out[0, 0]).all()
+    out[0, 0] = 0
+    assert torch.isfinite(out).all()
+
+
+def test_no_wait_gave_up(cuda_device):
+    """After everything above: no bounded wait of the prompt kernel has expired."""
+    from prime_kernels_b200 import _cabi
+
+    assert _cabi.library().pk_kv8_wait_timeouts() == 0
 
 
 def test_strides_and_shared_pages(cuda_device):
