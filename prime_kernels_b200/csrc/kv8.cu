@@ -71,7 +71,11 @@ __device__ __forceinline__ bool request_of(const Kv8Params& p, int t, int& r, in
 }
 
 // ---------------------------------------------------------------- append
-// One warp per (token, kv head); the first new token of a page leads and stores all new tokens of that page.
+// One warp per (16 consecutive rows, kv head), or per (request, kv head) with one token each.  Among its rows the warp
+// looks for the first new token of a page, which leads: it stores all new tokens of that page, K and V, whether or not
+// they lie among the warp's rows.  16 of them are kept in registers between the maximum and the values; more (pages of 32
+// slots and up) are read again, from L2.  Bound by bytes: 17.4 k tokens x 32 heads out of fused projection rows, 214 MB, in
+// 48 us; a warp per row, all but the leaders of which left at once, took 134 us.
 struct AppendParams {
     Kv8Params c;
     const uint16_t *k, *v;
@@ -89,69 +93,103 @@ __device__ __forceinline__ float amax8(const uint4 q) {
     return fmaxf(a, fmaxf(finite_abs(bf16_lo(q.w)), finite_abs(bf16_hi(q.w))));
 }
 
-__global__ void __launch_bounds__(256) kv8_append_kernel(AppendParams p) {
+__device__ __forceinline__ uint2 to_e4m3x8(const uint4 q, float inv) {
+    return make_uint2(e4m3x2(bf16_lo(q.x) * inv, bf16_hi(q.x) * inv) | (e4m3x2(bf16_lo(q.y) * inv, bf16_hi(q.y) * inv) << 16),
+                      e4m3x2(bf16_lo(q.z) * inv, bf16_hi(q.z) * inv) | (e4m3x2(bf16_lo(q.w) * inv, bf16_hi(q.w) * inv) << 16));
+}
+// The tokens of a page that are held already, after its scale grew: times f, a power of two.
+__device__ void rescale_page(uint8_t* dst, long long token_stride, int slots, float f, int lane) {
+    for (int i = lane >> 2; i < slots; i += 8) {
+        uint4* q = reinterpret_cast<uint4*>(dst + (long long)i * token_stride + (lane & 3) * 16);
+        uint4 a = *q;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t lo, hi;
+            e4m3x4_to_f16(w[j], lo, hi);
+            const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+            const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            w[j] = e4m3x2(fl.x * f, fl.y * f) | (e4m3x2(fh.x * f, fh.y * f) << 16);
+        }
+        *q = a;
+    }
+}
+
+template <int kGroup>
+__global__ void __launch_bounds__(256, kGroup == 1 ? 2 : 3) kv8_append_kernel(AppendParams p) {
     const Kv8Params& c = p.c;
     const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (item >= (long long)c.tokens * c.kv_heads) return;
-    const int t = (int)(item / c.kv_heads), h = (int)(item - (long long)t * c.kv_heads);
-    int r, first, count;
-    if (!request_of(c, t, r, first, count)) return;
-    const int size = 1 << c.page_shift;
-    const long long pos = (long long)c.seq_lens[r] - count + (t - first);
-    if (pos < 0) return;
-    const int slot = (int)(pos & (size - 1));
-    if (slot != 0 && t != first) return;               // another token of this page leads
-    const long long col = pos >> c.page_shift;
-    if (col >= c.bt_cols) return;
-    const int page = c.block_table[r * c.bt_stride + col];
-    if (page < 0 || page >= c.pages) return;
-    const int m = min(size - slot, first + count - t);
-    uint8_t* base = c.cache + (long long)page * c.page_stride + (long long)h * c.head_stride;
-    uint8_t* scale = c.scales + ((long long)page * c.kv_heads + h) * 2;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const uint16_t* src = x ? p.v + (long long)t * p.v_token + (long long)h * p.v_head
-                                : p.k + (long long)t * p.k_token + (long long)h * p.k_head;
-        const long long step = x ? p.v_token : p.k_token;
-        uint8_t* dst = base + (x ? c.v_off : c.k_off);
-        float amax = 0.f;
-        for (int i = lane >> 3; i < m; i += 4)
-            amax = fmaxf(amax, amax8(*reinterpret_cast<const uint4*>(src + i * step + (lane & 7) * 8)));
-        amax = warp_max(amax);
-        uint32_t e = e8m0_roundup(__fmul_rn(amax, 1.f / 448.f));
-        if (slot) {
-            const uint32_t old = min((uint32_t)scale[x], 254u);
-            if (e > old) {                             // the scale grows: values held move by 2^(old - e)
-                const float f = exp2_biased(127u - min(e - old, 126u));
-                for (int i = lane >> 2; i < slot; i += 8) {
-                    uint4* q = reinterpret_cast<uint4*>(dst + (long long)i * c.token_stride + (lane & 3) * 16);
-                    uint4 a = *q;
-                    uint32_t* w = reinterpret_cast<uint32_t*>(&a);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t lo, hi;
-                        e4m3x4_to_f16(w[j], lo, hi);
-                        const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                        const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                        w[j] = e4m3x2(fl.x * f, fl.y * f) | (e4m3x2(fh.x * f, fh.y * f) << 16);
-                    }
-                    *q = a;
-                }
-            } else {
-                e = old;
+    const long long group = item / c.kv_heads;
+    const int h = (int)(item - group * c.kv_heads), size = 1 << c.page_shift;
+    if (group * kGroup >= c.tokens) return;
+    // ---- lane i looks at row i of the group
+    const int mine = (int)group * kGroup + lane;
+    int slot = 0, m = 0, page = -1;
+    if (lane < kGroup && mine < c.tokens) {
+        int r, first, count;
+        if (request_of(c, mine, r, first, count)) {
+            const long long pos = (long long)c.seq_lens[r] - count + (mine - first);
+            slot = (int)(pos & (size - 1));
+            if (pos >= 0 && (slot == 0 || mine == first) && (pos >> c.page_shift) < c.bt_cols) {
+                page = c.block_table[r * c.bt_stride + (pos >> c.page_shift)];
+                m = min(size - slot, first + count - mine);
+                if (page >= c.pages) page = -1;
             }
         }
-        const float inv = exp2_biased(254u - e);
-        for (int i = lane >> 3; i < m; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(src + i * step + (lane & 7) * 8);
-            uint2 o;
-            o.x = e4m3x2(bf16_lo(q.x) * inv, bf16_hi(q.x) * inv) | (e4m3x2(bf16_lo(q.y) * inv, bf16_hi(q.y) * inv) << 16);
-            o.y = e4m3x2(bf16_lo(q.z) * inv, bf16_hi(q.z) * inv) | (e4m3x2(bf16_lo(q.w) * inv, bf16_hi(q.w) * inv) << 16);
-            *reinterpret_cast<uint2*>(dst + (long long)(slot + i) * c.token_stride + (lane & 7) * 8) = o;
+    }
+    for (unsigned leaders = __ballot_sync(kFullMask, page >= 0); leaders; leaders &= leaders - 1) {
+        const int who = __ffs(leaders) - 1;
+        const int t = (int)group * kGroup + who, s = __shfl_sync(kFullMask, slot, who), n = __shfl_sync(kFullMask, m, who);
+        const long long pg = __shfl_sync(kFullMask, page, who);
+        uint8_t* base = c.cache + pg * c.page_stride + (long long)h * c.head_stride;
+        uint8_t* scale = c.scales + (pg * c.kv_heads + h) * 2;
+        const uint16_t* k = p.k + (long long)t * p.k_token + (long long)h * p.k_head + (lane & 7) * 8;
+        const uint16_t* v = p.v + (long long)t * p.v_token + (long long)h * p.v_head + (lane & 7) * 8;
+        const int row = lane >> 3;                                           // of every four
+        constexpr int kQ = kGroup == 1 ? 1 : 4;                              // 16 tokens, a quarter of them a lane; or one
+        uint4 kq[kQ], vq[kQ];
+        auto load = [&](int from) {
+            const uint16_t *ka = k + (from + row) * p.k_token, *va = v + (from + row) * p.v_token;
+#pragma unroll
+            for (int i = 0; i < kQ; ++i, ka += 4 * p.k_token, va += 4 * p.v_token) {
+                const bool on = from + row + 4 * i < n;
+                kq[i] = on ? *reinterpret_cast<const uint4*>(ka) : make_uint4(0, 0, 0, 0);
+                vq[i] = on ? *reinterpret_cast<const uint4*>(va) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        float ka = 0.f, va = 0.f;
+        const int last = (n - 1) & ~15;
+        for (int from = 0; from <= last; from += 16) {
+            load(from);
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                ka = fmaxf(ka, amax8(kq[i]));
+                va = fmaxf(va, amax8(vq[i]));
+            }
         }
-        __syncwarp();
-        if (lane == 0) scale[x] = (uint8_t)e;
+        uint32_t ek = e8m0_roundup(__fmul_rn(warp_max(ka), 1.f / 448.f)), ev = e8m0_roundup(__fmul_rn(warp_max(va), 1.f / 448.f));
+        if (s) {                                                             // tokens are held: the scale may only grow
+            const uint32_t ok = min((uint32_t)scale[0], 254u), ov = min((uint32_t)scale[1], 254u);
+            if (ek > ok) rescale_page(base + c.k_off, c.token_stride, s, exp2_biased(127u - min(ek - ok, 126u)), lane);
+            if (ev > ov) rescale_page(base + c.v_off, c.token_stride, s, exp2_biased(127u - min(ev - ov, 126u)), lane);
+            ek = max(ek, ok);
+            ev = max(ev, ov);
+            __syncwarp();                                                    // the old scales have been read
+        }
+        const float ki = exp2_biased(254u - ek), vi = exp2_biased(254u - ev);
+        uint8_t* to = base + (long long)s * c.token_stride + (lane & 7) * 8;
+        for (int from = last; from >= 0; from -= 16) {                       // the last 16 are still in registers
+            if (from != last) load(from);
+            uint8_t* at = to + (from + row) * c.token_stride;
+#pragma unroll
+            for (int i = 0; i < kQ; ++i, at += 4 * c.token_stride)
+                if (from + row + 4 * i < n) {
+                    *reinterpret_cast<uint2*>(at + c.k_off) = to_e4m3x8(kq[i], ki);
+                    *reinterpret_cast<uint2*>(at + c.v_off) = to_e4m3x8(vq[i], vi);
+                }
+        }
+        if (lane == 0) *reinterpret_cast<uint16_t*>(scale) = (uint16_t)(ek | (ev << 8));
     }
 }
 
@@ -976,7 +1014,7 @@ int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     if ((long long)a->bt_cols * a->page_size > 0x7fffffffLL) return kErrMaxSeq;
     if (a->batch == 0 || tokens == 0) return -1;                             // nothing to do
     if (!a->cache || !a->scales || !a->seq_lens || (a->bt_cols > 0 && !a->block_table)) return kErrNull;
-    if (reinterpret_cast<uintptr_t>(a->cache) % 16 || a->k_off % 16 || a->v_off % 16 || a->page_stride % 16 ||
+    if (reinterpret_cast<uintptr_t>(a->cache) % 16 || reinterpret_cast<uintptr_t>(a->scales) % 2 || a->k_off % 16 || a->v_off % 16 || a->page_stride % 16 ||
         a->token_stride % 16 || a->head_stride % 16)
         return kErrAlign;
     if (!a->cu_seqlens && tokens < a->batch) return kErrShape;
@@ -1017,9 +1055,11 @@ extern "C" int pk_kv8_append(const PkKv8Cache* cache, const void* k, long long k
     p.v = static_cast<const uint16_t*>(v);
     p.k_token = k_token_stride; p.k_head = k_head_stride;
     p.v_token = v_token_stride; p.v_head = v_head_stride;
-    const long long blocks = ((long long)tokens * p.c.kv_heads + 7) / 8;
+    const int group = p.c.cu ? 16 : 1;
+    const long long blocks = (((long long)tokens + group - 1) / group * p.c.kv_heads + 7) / 8;
     if (blocks > 0x7fffffffLL) return kErrShape;
-    kv8_append_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    if (p.c.cu) kv8_append_kernel<16><<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    else kv8_append_kernel<1><<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return (int)cudaPeekAtLastError();
 }
 
