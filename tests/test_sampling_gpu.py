@@ -89,7 +89,7 @@ def test_settings_of_each_row(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("knobs", [{}, {"top_k": 3}, {"top_p": 0.6}, {"min_p": 0.2}, {"temperature": 0.0}])
+@pytest.mark.parametrize("knobs", [{}, {"top_k": 3}, {"top_k": 1}, {"top_k": 600}, {"top_p": 0.6}, {"min_p": 0.2}, {"min_p": 1.0}, {"temperature": 0.0}])
 def test_masked_and_special_logits(cuda_device, dtype, knobs):
     g = torch.Generator().manual_seed(8)
     t, vocab = TYPES[dtype], 700
@@ -111,6 +111,8 @@ def test_masked_and_special_logits(cuda_device, dtype, knobs):
     row(low, i77=0.0, i78=0.5)                         # a mask of lowest values
     row(None, i3=math.inf)                             # one infinity takes everything
     row(None, i3=math.inf, i600=math.inf)
+    row(math.inf)
+    row(-math.inf, i8=math.inf, i7=math.inf, i9=math.nan)
     row(0.0, i9=-0.0, i10=-0.0)                        # signed zeros are equal
     row(-0.0, i400=0.0)
     row(None, i0=math.nan, i699=-math.inf)
