@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/prime_kernels_b200.h"
@@ -259,6 +260,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
         "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -576,23 +583,25 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
 // ---------------------------------------------------------------- attention of many query tokens (prompt chunks)
 // The same rows and the same arithmetic with 128 rows a tile, on tcgen05: S = Q K^T (M 128, N 64, both operands K-major
 // in shared memory) and O += P V (P from tensor memory, V as it lies: [key][dim], MN-major), accumulators in tensor
-// memory.  One CTA holds one tile; warps 0-3 own a row a thread (softmax), warps 4-5 turn e4m3 pages into swizzled f16
-// tiles of 64 keys, one thread of warp 6 issues the products (eight warps, so that a thread may have 128 registers).  S is double-buffered, so the next scores are computed
+// memory.  One CTA holds one tile; warps 0-3 own a row a thread (softmax), warps 4-7 turn e4m3 pages into swizzled f16
+// tiles of 64 keys, and a thread of warp 7 issues the products: eight warps, two on each scheduler, 128 registers a thread.
+// (Two warps with all of the pages made the softmax warps beside them the slowest; sparing warp 7 its share made the other
+// three so: 259, 263 and 269 us where this takes 252.)  S is double-buffered, so the next scores are computed
 // while the softmax works, and two CTAs share an SM (256 columns of tensor memory each), so one's products run under
 // the other's exponentials.
 //
 // Bound by the exponentials: 16 a clock and SM against 64 x 4 flops each, a quarter of the tensor peak at head dim 64.
 // `top` is raised only where a row's maximum has grown by 2^8, so that the accumulator is rarely rescaled; f16 holds 2^8
 // times the weights.
-constexpr int kTileRows = 128, kTileKeys = 64, kPromptStages = 3;
-constexpr int kRawStages = 4, kRawBytes = kTileKeys * 128;              // e4m3 on its way
-constexpr int kPromptThreads = 256, kProducers = 64;
+constexpr int kTileRows = 128, kTileKeys = 64, kPromptStages = 4;
+constexpr int kRawStages = 3, kRawBytes = kTileKeys * 128;              // e4m3 on its way
+constexpr int kPromptThreads = 256, kProducers = 128;
 constexpr uint32_t kPromptCols = 256, kColP = 128, kColO = 192;            // S in columns 0..127, P in 128..191, two of each
 constexpr float kLazy = 8.f;
 
 struct PromptShared {
     uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full[2], pv_done[2], drain;
-    float ks[kPromptStages][4], ev[kPromptStages][4], bias[kPromptStages][4];   // per 16 keys; bias -inf: no page
+    __align__(16) float ks[kPromptStages][4], ev[kPromptStages][4], bias[kPromptStages][4];   // per 16 keys; bias -inf: no page
     uint32_t tmem;
     volatile int abort;
 };
@@ -601,7 +610,7 @@ constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileK
 __device__ unsigned int g_kv8_wait_timeouts;
 
 // Bounded wait: gives up after some seconds, or as soon as another thread of the CTA has.
-__device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ void prompt_poll(PromptShared& sh, uint64_t* bar, uint32_t parity) {
     for (uint32_t n = 0; n < (1u << 20); ++n) {
         if (mbar_test(bar, parity & 1u)) return;
         if ((n & 63) == 63 && sh.abort) return;
@@ -610,6 +619,9 @@ __device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uin
         sh.abort = 1;
         atomicAdd(&g_kv8_wait_timeouts, 1u);
     }
+}
+__device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
+    if (__builtin_expect(!mbar_test(bar, parity & 1u), 0)) prompt_poll(sh, bar, parity);
 }
 // The same for a whole warp whose next instruction is a warp-wide one: lanes may leave the polling loop apart.
 __device__ __forceinline__ void warp_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
@@ -707,7 +719,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 6) {
+    if (warp == 7) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(kPromptCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -764,8 +776,12 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 float s[kTileKeys];
                 tmem_ld32(lanes + (at & 1) * kTileKeys, s);
                 tmem_ld32(lanes + (at & 1) * kTileKeys + 32, s + 32);
+                const float4 ks4 = *reinterpret_cast<const float4*>(sh.ks[stage]), ev4 = *reinterpret_cast<const float4*>(sh.ev[stage]),
+                             bias4 = *reinterpret_cast<const float4*>(sh.bias[stage]);
+                const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w}, ev[4] = {ev4.x, ev4.y, ev4.z, ev4.w},
+                            bias[4] = {bias4.x, bias4.y, bias4.z, bias4.w};
                 tmem_ld_wait();
-                if (i * kTileKeys + kTileKeys > len_min) {
+                if (__builtin_expect(i * kTileKeys + kTileKeys > len_min, 0)) {
                     const int left = len - i * kTileKeys;                  // scores from here on are masked
 #pragma unroll
                     for (int k = 0; k < kTileKeys; ++k)
@@ -780,10 +796,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
 #pragma unroll
                     for (int k = 0; k < 3; ++k) mx[k] = max3(mx[k], s[16 * u + 5 * k + 3], s[16 * u + 5 * k + 4]);
                     mx[0] = fmaxf(max3(mx[0], mx[1], mx[2]), s[16 * u + 15]);
-                    ck[u] = fmaxf(sh.ks[stage][u] * qs, 1e-37f);           // never 0: a masked score times it stays -inf
-                    const float x = fmaf(mx[0], ck[u], sh.bias[stage][u]);
+                    ck[u] = fmaxf(ks[u] * qs, 1e-37f);           // never 0: a masked score times it stays -inf
+                    const float x = fmaf(mx[0], ck[u], bias[u]);
                     m1 = fmaxf(m1, x);
-                    t1 = fmaxf(t1, x + sh.ev[stage][u]);
+                    t1 = fmaxf(t1, x + ev[u]);
                 }
                 const float mu = m1 == kNegInf ? 0.f : m1;
                 l *= ex2(m - mu);
@@ -796,59 +812,45 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 const float tu = top == kNegInf ? 0.f : top;
                 // weights straight as 2^(s + ev - top), their sum put back to 2^(s - m); a page whose V scale is so small that
                 // its weights vanish (a page of zeros) still counts in the sum: in two steps there
+                // all arguments, the exponentials of the first half, those of the second between the first's uses: the
+                // exponential unit is what the others wait for
+                float f[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) f[u] = ex2(fminf(mu + ev[u] - tu, 127.f));       // 2^(s - m) -> 2^(s + ev - top)
+#pragma unroll
+                for (int k = 0; k < kTileKeys; k += 2) {
+                    const float to_m = bias[k / 16] - mu;
+                    const float2 x = fma2(make_float2(s[k], s[k + 1]), make_float2(ck[k / 16], ck[k / 16]), make_float2(to_m, to_m));
+                    s[k] = x.x;
+                    s[k + 1] = x.y;
+                }
+#pragma unroll
+                for (int k = 0; k < 32; ++k) s[k] = ex2(s[k]);
+                float2 sum[4] = {};
+                uint32_t pk[16];
+                auto use = [&](int k) {                                    // keys k, k + 1
+                    const float2 e = make_float2(s[k], s[k + 1]);
+                    sum[k / 16] = add2(sum[k / 16], e);
+                    const float2 w = mul2(e, make_float2(f[k / 16], f[k / 16]));
+                    pk[k / 2 % 16] = pack_f16x2(w.x, w.y);
+                };
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    s[32 + k] = ex2(s[32 + k]);
+                    s[33 + k] = ex2(s[33 + k]);
+                    use(k);
+                }
                 if (i > 1) {                                               // this P has been read
                     warp_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
                     tc_fence_after();
                 }
+                tmem_st16(lanes + kColP + (at & 1) * 32, pk);
 #pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    float shift[2], lf[2];
+                for (int k = 32; k < kTileKeys; k += 2) use(k);
+                tmem_st16(lanes + kColP + (at & 1) * 32 + 16, pk);
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const float ev = sh.ev[stage][2 * d + v];
-                        lf[v] = mu + ev - tu;
-                        shift[v] = sh.bias[stage][2 * d + v] + ev - tu;
-                    }
-                    uint32_t pk[16];
-                    if (__all_sync(kFullMask, fminf(lf[0], lf[1]) > -60.f)) {
-                        // in the order that hides the exponentials' latency: all arguments, all exponentials, then their uses
-#pragma unroll
-                        for (int k = 0; k < 32; k += 2) {
-                            const float2 x = fma2(make_float2(s[32 * d + k], s[32 * d + k + 1]), make_float2(ck[2 * d + k / 16], ck[2 * d + k / 16]),
-                                                  make_float2(shift[k / 16], shift[k / 16]));
-                            s[32 * d + k] = x.x;
-                            s[32 * d + k + 1] = x.y;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) s[32 * d + k] = ex2(s[32 * d + k]);
-#pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            float2 sum = make_float2(s[32 * d + 16 * v], s[32 * d + 16 * v + 1]);
-                            pk[8 * v] = pack_f16x2(s[32 * d + 16 * v], s[32 * d + 16 * v + 1]);
-#pragma unroll
-                            for (int k = 2; k < 16; k += 2) {
-                                sum = add2(sum, make_float2(s[32 * d + 16 * v + k], s[32 * d + 16 * v + k + 1]));
-                                pk[8 * v + k / 2] = pack_f16x2(s[32 * d + 16 * v + k], s[32 * d + 16 * v + k + 1]);
-                            }
-                            l = fmaf(sum.x + sum.y, ex2(-lf[v]), l);
-                        }
-                    } else {
-#pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            const float f = ex2(fminf(lf[v], 127.f)), to_m = sh.bias[stage][2 * d + v] - mu;
-                            float sum = 0.f;
-#pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                const float a = ex2(fmaf(s[32 * d + 16 * v + k], ck[2 * d + v], to_m)), b = ex2(fmaf(s[32 * d + 16 * v + k + 1], ck[2 * d + v], to_m));
-                                sum += a + b;
-                                pk[8 * v + k / 2] = pack_f16x2(a * f, b * f);
-                            }
-                            l += sum;
-                        }
-                    }
-                    tmem_st16(lanes + kColP + (at & 1) * 32 + 16 * d, pk);
-                }
-                if (i > 0 && __any_sync(kFullMask, turn != 1.f)) {
+                for (int u = 0; u < 4; ++u) l += sum[u].x + sum[u].y;
+                if (__builtin_expect(i > 0 && __any_sync(kFullMask, turn != 1.f), 0)) {
                     warp_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
                     tc_fence_after();
 #pragma unroll
@@ -893,41 +895,42 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
             }
             if (on && p.lse) p.lse[(long long)(first + tok) * p.q_heads + head] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
             tc_fence_before();                                             // the accumulator is read: the next tile may write it
-        } else if (warp < 6) {
-            // ---------------- e4m3 pages to f16 tiles: a thread carries 16 bytes of one K row and of one V row of each unit of
-            // 16 keys; the pages of the next 32 units (8 steps) and their scales are held one a lane
-            const int pid = tid - 128, key = pid >> 2, part = pid & 3;
-            static_assert(kProducers == 64 && kTileKeys == 64, "16 rows of four parts: one unit");
+        } else {
+            // ---------------- e4m3 pages to f16 tiles: a warp carries 16 keys of each step, a lane 16 bytes of two K rows and
+            // of two V rows; the pages of the warp's next 32 steps and their scales are held one a lane.  The last warp issues
+            // the products as well.
+            const int unit = warp - 4, key = lane >> 2, part = lane & 3;
+            static_assert(kProducers == 128 && kTileKeys == 64, "four warps, a quarter of a tile each");
             const uint8_t* from = c.cache + (long long)h * c.head_stride + c.k_off + key * c.token_stride + 16 * part;
-            const long long v_from_k = c.v_off - c.k_off;
+            const long long v_from_k = c.v_off - c.k_off, eight = 8 * c.token_stride;
             const int in_page = (1 << c.page_shift) - 1;
-            unsigned char* mine = raw_ring + pid * 16;                     // K parts, then V parts; read back by their writer
-            const uint32_t lo_at = key * 128 + ((2 * part) ^ (key & 7)) * 16, hi_at = key * 128 + ((2 * part + 1) ^ (key & 7)) * 16;
-            int pages = -1;
-            uint32_t scale2 = 0, used_scale2 = 0;                          // of the units being fetched, being converted
-            int used_pages = -1;
+            unsigned char* mine = raw_ring + (tid - 128) * 16;             // two K rows, two V rows; read back by their writer
+            const uint32_t lo_at = (16 * unit + key) * 128 + ((2 * part) ^ key) * 16, hi_at = (16 * unit + key) * 128 + ((2 * part + 1) ^ key) * 16;
+            int pages = -1, used_pages = -1;                               // of the steps being fetched, being converted
+            uint32_t scale2 = 0, used_scale2 = 0;
             auto fetch = [&](int i) {
-                if ((i & 7) == 0) {
-                    const int unit = 4 * i + lane;
+                const int at = i * kTileKeys + 16 * unit;
+                if ((i & 31) == 0) {
+                    const int first_key = at + lane * kTileKeys;
                     used_pages = pages;
                     used_scale2 = scale2;
-                    pages = unit * 16 < len_max ? table[unit * 16 >> c.page_shift] : -1;
+                    pages = first_key < len_max ? table[first_key >> c.page_shift] : -1;
                     if (pages >= c.pages || pages < 0) pages = -1;
                     scale2 = pages < 0 ? 0u : *reinterpret_cast<const uint16_t*>(c.scales + ((long long)pages * c.kv_heads + h) * 2);
                 }
+                const int page = __shfl_sync(kFullMask, pages, i & 31);
+                const int left = page < 0 ? 0 : len_max - at;
+                const uint8_t* src = from + (page < 0 ? 0 : (long long)page * c.page_stride + (long long)(at & in_page) * c.token_stride);
                 unsigned char* to = mine + (i % kRawStages) * kRawBytes;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int page = __shfl_sync(kFullMask, pages, (4 * i + u) & 31), at = i * kTileKeys + 16 * u;
-                    const bool live = page >= 0 && at + key < len_max;
-                    const uint8_t* src = from + (live ? (long long)page * c.page_stride + (long long)(at & in_page) * c.token_stride : 0);
-                    cp_async16(to + u * kProducers * 16, src, live);
-                    cp_async16(to + (4 + u) * kProducers * 16, src + v_from_k, live);
-                }
+                const bool on0 = key < left, on1 = key + 8 < left;
+                const uint8_t *src0 = on0 ? src : from, *src1 = on1 ? src + eight : from;
+                cp_async16(to, src0, on0);
+                cp_async16(to + kProducers * 16, src1, on1);
+                cp_async16(to + 2 * kProducers * 16, src0 + v_from_k, on0);
+                cp_async16(to + 3 * kProducers * 16, src1 + v_from_k, on1);
                 cp_async_commit();
             };
-            for (int i = 0; i < kRawStages - 1; ++i) fetch(i);
-            for (int i = 0; i < steps; ++i) {
+            auto produce = [&](int i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
                 fetch(i + kRawStages - 1);                                 // steps past the last fetch zeros
                 cp_async_wait<kRawStages - 1>();
@@ -935,9 +938,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 unsigned char* k_tile = kv_tiles + stage * 2 * kTileKeys * 128;
                 const unsigned char* raw16 = mine + (i % kRawStages) * kRawBytes;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     const uint4 v = *reinterpret_cast<const uint4*>(raw16 + j * kProducers * 16);
-                    unsigned char* to = k_tile + j * 16 * 128;             // four units of K, then of V
+                    unsigned char* to = k_tile + (j >> 1) * kTileKeys * 128 + (j & 1) * 8 * 128;
                     uint4 lo, hi;
                     e4m3x4_to_f16(v.x, lo.x, lo.y);
                     e4m3x4_to_f16(v.y, lo.z, lo.w);
@@ -946,50 +949,63 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                     *reinterpret_cast<uint4*>(to + lo_at) = lo;
                     *reinterpret_cast<uint4*>(to + hi_at) = hi;
                 }
-                const bool older = ((i + kRawStages - 1) & ~7) != (i & ~7);
-                if (warp == 4 && (lane >> 2) == (i & 7)) {
+                const bool older = ((i + kRawStages - 1) & ~31) != (i & ~31);
+                if (lane == (i & 31)) {
                     const bool none = (older ? used_pages : pages) < 0;
                     const uint32_t two = older ? used_scale2 : scale2;
-                    sh.ks[stage][lane & 3] = exp2_biased(two & 0xffu);
-                    sh.ev[stage][lane & 3] = (float)(int)(two >> 8) - 127.f;
-                    sh.bias[stage][lane & 3] = none ? kNegInf : 0.f;
+                    sh.ks[stage][unit] = exp2_biased(two & 0xffu);
+                    sh.ev[stage][unit] = (float)(int)(two >> 8) - 127.f;
+                    sh.bias[stage][unit] = none ? kNegInf : 0.f;
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.full[stage]);
+            };
+            for (int i = 0; i < kRawStages - 1; ++i) fetch(i);
+            if (warp < 7) {
+                for (int i = 0; i < steps; ++i) produce(i);
+            } else {
+                const uint64_t dq = tile_desc(q_tile);
+                auto scores = [&](int i) {
+                    const uint32_t at = n + i, stage = at % kPromptStages;
+                    prompt_wait(sh, &sh.full[stage], at / kPromptStages);
+                    tc_fence_after();
+                    const uint64_t dk = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)                            // 16 dims = 32 bytes a product
+                        mma_ss(tmem + (at & 1) * kTileKeys, dq + 2 * k, dk + 2 * k, kIdescQK, k > 0);
+                    mma_commit(&sh.s_full[at & 1]);
+                    mbar_arrive(&sh.s_full[at & 1]);                       // hands on the scales that came with the tile
+                };
+                // two tiles ahead of the products: a tile's stage is free once the products of four steps before are done
+                for (int i = 0; i < min(2, steps); ++i) produce(i);
+                if (lane == 0) {
+                    prompt_wait(sh, &sh.q_full, tiles_done);
+                    if (steps > 0) scores(0);
+                }
+                __syncwarp();
+                for (int i = 0; i < steps; ++i) {
+                    if (lane == 0 && i + 1 < steps) scores(i + 1);
+                    __syncwarp();
+                    if (i + 2 < steps) produce(i + 2);
+                    if (lane == 0) {
+                        const uint32_t at = n + i, stage = at % kPromptStages;
+                        prompt_wait(sh, &sh.p_full[at & 1], at >> 1);
+                        tc_fence_after();
+                        const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)                        // 16 keys = 2048 bytes of V, 8 columns of P
+                            mma_ts(tmem + kColO, tmem + kColP + (at & 1) * 32 + 8 * k, dv + 128 * k, kIdescPV, i > 0 || k > 0);
+                        mma_commit(&sh.empty[stage]);
+                        mma_commit(&sh.pv_done[at & 1]);
+                    }
+                    __syncwarp();
+                }
             }
             cp_async_wait<0>();                                            // the next tile's copies go to the same places
-        } else if (warp == 6 && lane == 0) {
-            // ---------------- products
-            prompt_wait(sh, &sh.q_full, tiles_done);
-            const uint64_t dq = tile_desc(q_tile);
-            auto scores = [&](int i) {
-                const uint32_t at = n + i, stage = at % kPromptStages;
-                prompt_wait(sh, &sh.full[stage], at / kPromptStages);
-                tc_fence_after();
-                const uint64_t dk = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)                                // 16 dims = 32 bytes a product
-                    mma_ss(tmem + (at & 1) * kTileKeys, dq + 2 * k, dk + 2 * k, kIdescQK, k > 0);
-                mma_commit(&sh.s_full[at & 1]);
-                mbar_arrive(&sh.s_full[at & 1]);                           // hands on the scales that came with the tile
-            };
-            if (steps > 0) scores(0);
-            for (int i = 0; i < steps; ++i) {
-                const uint32_t at = n + i, stage = at % kPromptStages;
-                if (i + 1 < steps) scores(i + 1);
-                prompt_wait(sh, &sh.p_full[at & 1], at >> 1);
-                tc_fence_after();
-                const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)                                // 16 keys = 2048 bytes of V, 8 columns of P
-                    mma_ts(tmem + kColO, tmem + kColP + (at & 1) * 32 + 8 * k, dv + 128 * k, kIdescPV, i > 0 || k > 0);
-                mma_commit(&sh.empty[stage]);
-                mma_commit(&sh.pv_done[at & 1]);
-            }
         }
         n += (uint32_t)steps;
     }
-    if (warp == 6) {
+    if (warp == 7) {
         if (lane == 0) {                                                   // nothing is in flight when the memory goes
             mma_commit(&sh.drain);
             prompt_wait(sh, &sh.drain, 0);
@@ -999,10 +1015,23 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 6) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPromptCols) : "memory");
+    if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPromptCols) : "memory");
 }
 
 // ---------------------------------------------------------------- host
+// The dynamic shared memory a kernel may have is set once per device, not before every launch.
+template <typename K> cudaError_t allow_shared(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+std::atomic<unsigned long long> g_prompt_ready{0}, g_attend_ready[2];
+
 int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     if (!a) return kErrNull;
     if (a->batch < 0 || a->batch > 65535 || tokens < 0 || a->kv_heads <= 0 || a->kv_heads > 65535 || a->pages < 0 ||
@@ -1096,7 +1125,7 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     if (small >= 740 && 10 * small >= 36 * ((expected + kTileRows - 1) / kTileRows) * sets) {
         const long long tiles = ((long long)longest * p.group + kTileRows - 1) / kTileRows;
         p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
-        const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPromptBytes);
+        const cudaError_t e = allow_shared(kv8_prompt_kernel, kPromptBytes, g_prompt_ready);
         if (e != cudaSuccess) return (int)e;
         kv8_prompt_kernel<<<dim3((unsigned)p.tiles, (unsigned)p.c.kv_heads, (unsigned)p.c.batch), kPromptThreads, kPromptBytes,
                             static_cast<cudaStream_t>(stream)>>>(p);
@@ -1129,6 +1158,6 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     cfg.attrs = at;
     cfg.numAttrs = 1;
     const auto kernel = tile_rows == 8 ? kv8_attend_kernel<true> : kv8_attend_kernel<false>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttShared);
+    const cudaError_t e = allow_shared(kernel, kAttShared, g_attend_ready[tile_rows == 8]);
     return (int)(e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, p));
 }

@@ -31,6 +31,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/prime_kernels_b200.h"
@@ -413,6 +414,8 @@ __device__ __noinline__ void radix_border(SampleShared& sh, const typename KeyOf
 }
 
 constexpr size_t kSampleShared = (sizeof(SampleShared) + 15) / 16 * 16;
+constexpr int kSampleMost = 227 * 1024;                    // a block's shared memory
+static_assert(kSampleShared + (size_t)kSampleMaxVocab / kMaxCluster * 4 <= kSampleMost, "the largest slice fits");
 
 template <int DT>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams p) {
@@ -860,8 +863,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
 
 template <int DT>
 int launch_sample(const SampleParams& p, int rows, int cluster, size_t smem, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the dynamic shared memory a launch may have, set once per device to the most one can need
+    static std::atomic<unsigned long long> ready{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!(ready.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleMost);
+        if (e != cudaSuccess) return (int)e;
+        ready.fetch_or(bit, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
     cfg.blockDim = dim3(kSampleThreads);

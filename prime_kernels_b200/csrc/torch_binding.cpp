@@ -352,16 +352,12 @@ void kv8_attention_out(const torch::Tensor& q, const torch::Tensor& cache, const
     TORCH_CHECK(rc == 0, "kv8 attention failed: ", pk_status_string(rc));
 }
 
-std::tuple<torch::Tensor, torch::Tensor> kv8_attention(const torch::Tensor& q, const torch::Tensor& cache,
-                                                       const torch::Tensor& scales, const torch::Tensor& block_table,
-                                                       const torch::Tensor& seq_lens, const std::optional<torch::Tensor>& cu_seqlens,
-                                                       int64_t max_query_len, double scale, bool return_lse) {
+torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& cache, const torch::Tensor& scales,
+                            const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                            const std::optional<torch::Tensor>& cu_seqlens, int64_t max_query_len, double scale) {
     torch::Tensor out = torch::empty(q.sizes(), q.options());
-    torch::Tensor lse = return_lse && q.dim() == 3 ? torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32))
-                                                   : torch::empty({0}, q.options().dtype(torch::kFloat32));
-    kv8_attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, out,
-                      return_lse ? std::optional<torch::Tensor>(lse) : std::nullopt);
-    return {out, lse};
+    kv8_attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, out, std::nullopt);
+    return out;
 }
 
 // ---- sampling
@@ -409,18 +405,15 @@ void sample_out(const torch::Tensor& logits, const torch::Tensor& uniform, const
     TORCH_CHECK(rc == 0, "sample failed: ", pk_status_string(rc));
 }
 
-std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits, const torch::Tensor& uniform,
-                                                const std::optional<torch::Tensor>& temperature, double temperature_value,
-                                                const std::optional<torch::Tensor>& top_k, int64_t top_k_value,
-                                                const std::optional<torch::Tensor>& top_p, double top_p_value,
-                                                const std::optional<torch::Tensor>& min_p, double min_p_value, bool return_logprobs) {
+torch::Tensor sample(const torch::Tensor& logits, const torch::Tensor& uniform, const std::optional<torch::Tensor>& temperature,
+                     double temperature_value, const std::optional<torch::Tensor>& top_k, int64_t top_k_value,
+                     const std::optional<torch::Tensor>& top_p, double top_p_value, const std::optional<torch::Tensor>& min_p,
+                     double min_p_value) {
     TORCH_CHECK(logits.dim() == 2, "logits must be a CUDA tensor [rows, vocab]");
-    auto opts = torch::TensorOptions().device(logits.device());
-    torch::Tensor ids = torch::empty({logits.size(0)}, opts.dtype(torch::kInt64));
-    torch::Tensor lp = torch::empty({return_logprobs ? logits.size(0) : 0}, opts.dtype(torch::kFloat32));
+    torch::Tensor ids = torch::empty({logits.size(0)}, torch::TensorOptions().device(logits.device()).dtype(torch::kInt64));
     sample_out(logits, uniform, temperature, temperature_value, top_k, top_k_value, top_p, top_p_value, min_p, min_p_value, ids,
-               return_logprobs ? std::optional<torch::Tensor>(lp) : std::nullopt);
-    return {ids, lp};
+               std::nullopt);
+    return ids;
 }
 
 }  // namespace
@@ -430,7 +423,7 @@ TORCH_LIBRARY_FRAGMENT(prime_kv8, m) {
           "Tensor? cu_seqlens) -> ()");
     m.impl("append", torch::kCUDA, &kv8_append);
     m.def("attention(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
-          "int max_query_len, float scale, bool return_lse) -> (Tensor, Tensor)");
+          "int max_query_len, float scale) -> Tensor");
     m.impl("attention", torch::kCUDA, &kv8_attention);
     m.def("attention_out(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
           "int max_query_len, float scale, Tensor(a!) out, Tensor(b!)? lse) -> ()");
@@ -439,7 +432,7 @@ TORCH_LIBRARY_FRAGMENT(prime_kv8, m) {
 
 TORCH_LIBRARY_FRAGMENT(prime_sampling, m) {
     m.def("sample(Tensor logits, Tensor uniform, Tensor? temperature, float temperature_value, Tensor? top_k, int top_k_value, "
-          "Tensor? top_p, float top_p_value, Tensor? min_p, float min_p_value, bool return_logprobs) -> (Tensor, Tensor)");
+          "Tensor? top_p, float top_p_value, Tensor? min_p, float min_p_value) -> Tensor");
     m.impl("sample", torch::kCUDA, &sample);
     m.def("sample_out(Tensor logits, Tensor uniform, Tensor? temperature, float temperature_value, Tensor? top_k, int top_k_value, "
           "Tensor? top_p, float top_p_value, Tensor? min_p, float min_p_value, Tensor(a!) ids, Tensor(b!)? logprobs) -> ()");

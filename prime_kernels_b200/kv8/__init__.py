@@ -34,9 +34,8 @@ def _append_fake(k, v, cache, scales, block_table, seq_lens, cu_seqlens):
 
 
 @torch.library.register_fake("prime_kv8::attention")
-def _attention_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, return_lse):
-    return (q.new_empty(q.shape),
-            torch.empty(q.shape[:2] if return_lse else (0,), dtype=torch.float32, device=q.device))
+def _attention_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale):
+    return q.new_empty(q.shape)
 
 
 @torch.library.register_fake("prime_kv8::attention_out")
@@ -79,8 +78,9 @@ def attention(q, cache, scales, block_table, seq_lens, cu_seqlens=None, *, max_q
     With ``out`` given, rows that belong to no request are left as they are there; otherwise they are undefined."""
     n, s = max_query_len or 0, HEAD_DIM ** -0.5 if scale is None else scale
     if out is None:
-        o, lse = _attention(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s, return_lse)
-        return (o, lse) if return_lse else o
+        if not return_lse:
+            return _attention(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s, out, lse)
     return (out, lse) if return_lse else out

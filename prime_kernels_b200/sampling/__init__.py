@@ -27,11 +27,8 @@ MAX_VOCAB = 262144
 
 
 @torch.library.register_fake("prime_sampling::sample")
-def _sample_fake(logits, uniform, temperature, temperature_value, top_k, top_k_value, top_p, top_p_value, min_p, min_p_value,
-                 return_logprobs):
-    rows = logits.shape[0]
-    return (torch.empty((rows,), dtype=torch.int64, device=logits.device),
-            torch.empty((rows if return_logprobs else 0,), dtype=torch.float32, device=logits.device))
+def _sample_fake(logits, uniform, temperature, temperature_value, top_k, top_k_value, top_p, top_p_value, min_p, min_p_value):
+    return torch.empty((logits.shape[0],), dtype=torch.int64, device=logits.device)
 
 
 @torch.library.register_fake("prime_sampling::sample_out")
@@ -75,8 +72,9 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
         m, min_p = min_p, 0.0
     _check(temperature, top_k, top_p, min_p)
     if out is None:
-        ids, lp = _sample(logits, uniform, t, temperature, k, top_k, p, top_p, m, min_p, return_logprobs)
-        return (ids, lp) if return_logprobs else ids
+        if not return_logprobs:
+            return _sample(logits, uniform, t, temperature, k, top_k, p, top_p, m, min_p)
+        out = torch.empty((logits.shape[0],), dtype=torch.int64, device=logits.device)
     lp = torch.empty((logits.shape[0],), dtype=torch.float32, device=logits.device) if return_logprobs else None
     _sample_out(logits, uniform, t, temperature, k, top_k, p, top_p, m, min_p, out, lp)
     return (out, lp) if return_logprobs else out
