@@ -76,22 +76,33 @@ __device__ __forceinline__ bool request_of(const Kv8Params& p, int t, int& r, in
 // looks for the first new token of a page, which leads: it stores all new tokens of that page, K and V, whether or not
 // they lie among the warp's rows.  16 of them are kept in registers between the maximum and the values; more (pages of 32
 // slots and up) are read again, from L2.  Bound by bytes: 17.4 k tokens x 32 heads out of fused projection rows, 214 MB, in
-// 48 us; a warp per row, all but the leaders of which left at once, took 134 us.
+// 43 us (0.76 of the measured copy bandwidth); a warp per row, all but the leaders of which left at once, took 134 us.
 struct AppendParams {
     Kv8Params c;
     const uint16_t *k, *v;
     long long k_token, k_head, v_token, v_head;        // elements
 };
 
-__device__ __forceinline__ float finite_abs(float x) {
-    x = fabsf(x);
-    return x < __int_as_float(0x7f800000) ? x : 0.f;   // NaN and Inf do not count
-}
-__device__ __forceinline__ float amax8(const uint4 q) {
-    float a = fmaxf(finite_abs(bf16_lo(q.x)), finite_abs(bf16_hi(q.x)));
-    a = fmaxf(a, fmaxf(finite_abs(bf16_lo(q.y)), finite_abs(bf16_hi(q.y))));
-    a = fmaxf(a, fmaxf(finite_abs(bf16_lo(q.z)), finite_abs(bf16_hi(q.z))));
-    return fmaxf(a, fmaxf(finite_abs(bf16_lo(q.w)), finite_abs(bf16_hi(q.w))));
+// Largest finite magnitude of bf16 values, as its 15 bits: magnitudes are ordered like their bits, two to a word.
+template <int kQ> __device__ __forceinline__ uint32_t amax_bits(const uint4 (&q)[kQ]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+        m = __vmaxu2(m, __vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu));
+        m = __vmaxu2(m, __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
+    }
+    m = max(m & 0xffffu, m >> 16);
+    if (m >= 0x7f80u) {                                // NaN and Inf do not count
+        m = 0;
+        for (int i = 0; i < kQ; ++i) {
+            const uint32_t w[4] = {q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu, q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu};
+            for (int j = 0; j < 4; ++j) {
+                if ((w[j] & 0xffffu) < 0x7f80u) m = max(m, w[j] & 0xffffu);
+                if ((w[j] >> 16) < 0x7f80u) m = max(m, w[j] >> 16);
+            }
+        }
+    }
+    return m;
 }
 
 __device__ __forceinline__ uint2 to_e4m3x8(const uint4 q, float inv) {
@@ -159,17 +170,15 @@ __global__ void __launch_bounds__(256, kGroup == 1 ? 2 : 3) kv8_append_kernel(Ap
                 vq[i] = on ? *reinterpret_cast<const uint4*>(va) : make_uint4(0, 0, 0, 0);
             }
         };
-        float ka = 0.f, va = 0.f;
+        uint32_t ka = 0, va = 0;
         const int last = (n - 1) & ~15;
         for (int from = 0; from <= last; from += 16) {
             load(from);
-#pragma unroll
-            for (int i = 0; i < kQ; ++i) {
-                ka = fmaxf(ka, amax8(kq[i]));
-                va = fmaxf(va, amax8(vq[i]));
-            }
+            ka = max(ka, amax_bits(kq));
+            va = max(va, amax_bits(vq));
         }
-        uint32_t ek = e8m0_roundup(__fmul_rn(warp_max(ka), 1.f / 448.f)), ev = e8m0_roundup(__fmul_rn(warp_max(va), 1.f / 448.f));
+        auto scale_of = [](uint32_t bits) { return e8m0_roundup(__fmul_rn(__uint_as_float(__reduce_max_sync(kFullMask, bits) << 16), 1.f / 448.f)); };
+        uint32_t ek = scale_of(ka), ev = scale_of(va);
         if (s) {                                                             // tokens are held: the scale may only grow
             const uint32_t ok = min((uint32_t)scale[0], 254u), ov = min((uint32_t)scale[1], 254u);
             if (ek > ok) rescale_page(base + c.k_off, c.token_stride, s, exp2_biased(127u - min(ek - ok, 126u)), lane);
