@@ -84,13 +84,13 @@ struct AppendParams {
 };
 
 // Largest finite magnitude of bf16 values, as its 15 bits: magnitudes are ordered like their bits, two to a word.
+__device__ __forceinline__ uint32_t amax_two(const uint4 q) {             // of eight, in two halves
+    return __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu), __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+}
 template <int kQ> __device__ __forceinline__ uint32_t amax_bits(const uint4 (&q)[kQ]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-        m = __vmaxu2(m, __vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu));
-        m = __vmaxu2(m, __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
-    }
+    for (int i = 0; i < kQ; ++i) m = __vmaxu2(m, amax_two(q[i]));
     m = max(m & 0xffffu, m >> 16);
     if (m >= 0x7f80u) {                                // NaN and Inf do not count
         m = 0;
@@ -215,7 +215,11 @@ __global__ void __launch_bounds__(256, kGroup == 1 ? 2 : 3) kv8_append_kernel(Ap
 //
 // V scales differ from page to page, so weights enter the second product as 2^(s + eV - top) with a running maximum
 // `top` of s + eV of their own, apart from the running maximum of s that the sum uses: neither over- nor underflows
-// whatever the scales are.
+// whatever the scales are, as long as 2^(s - m) does not.
+//
+// A key that only later tokens of a tile see has weight 0 for the others, and 0 * NaN is NaN: where rows of a tile differ
+// in what they see, NaN among the V values is taken for 0 in the product and put into the rows that see it at the end
+// (the prompt kernel computes rows that it spoiled once more).
 //
 // Bound by the bytes of the cache where there are many, by the chain of dependent reads at the start (length, page, page's
 // data) and the merge where there are few.  64 requests of up to 8192 tokens, 15/5 heads: 44 us, 4.8 TB/s, 0.73 of the
@@ -241,6 +245,7 @@ constexpr float kNegInf = -__builtin_huge_valf();
 struct __align__(16) AttendShared {
     float o[16][kHeadDim + 4];
     float m[16], top[16], l[16];                       // running maxima (log2) and sum
+    int nan_seen;
 };
 
 static_assert(sizeof(AttendShared) <= kStages * kStageBytes, "the merge reuses the rings");
@@ -295,6 +300,26 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// NaN of e4m3 (0x7f, 0xff) among four values: 0x80 in each such byte
+__device__ __forceinline__ uint32_t e4m3_nan(uint32_t four) { return ((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// the four values with 0 for NaN; `seen` collects
+__device__ __forceinline__ uint32_t without_nan(uint32_t four, uint32_t& seen) {
+    const uint32_t nan = e4m3_nan(four);
+    seen |= nan;
+    return four & ~((nan >> 7) * 0xffu);
+}
+// Output dims of a row that are NaN because a V value among the keys from..len - 1, all of which it sees, is: dims
+// d0..d0 + n - 1 of `to`.
+__device__ __noinline__ void put_nan(const Kv8Params& c, const int* table, int h, int from, int len, uint16_t* to, int d0, int n) {
+    for (int key = from; key < len; ++key) {
+        const int page = table[key >> c.page_shift];
+        if (page < 0 || page >= c.pages) continue;
+        const uint8_t* v = c.cache + (long long)page * c.page_stride + (long long)h * c.head_stride + c.v_off +
+                           (long long)(key & ((1 << c.page_shift) - 1)) * c.token_stride;
+        for (int d = d0; d < d0 + n; ++d)
+            if ((v[d] & 0x7f) == 0x7f) to[d] = 0x7fff;
+    }
+}
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(kFullMask, v, 1));
     return fmaxf(v, __shfl_xor_sync(kFullMask, v, 2));
@@ -347,7 +372,7 @@ template <int kPer> struct Merged {
 // kHalf: tiles of 8 rows (a decode step of up to 8 query heads per kv head): the lower half of the 16-row operand is
 // empty and its softmax is left out.
 template <bool kHalf>
-__global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_kernel(AttendParams p) {
+__global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_kernel(const __grid_constant__ AttendParams p) {
     constexpr int kRows = kHalf ? 8 : 16, kR = kHalf ? 1 : 2;              // rows of a tile, of a lane
     const Kv8Params& c = p.c;
     cg::cluster_group cluster = cg::this_cluster();
@@ -429,6 +454,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
 #pragma unroll
         for (int i = 0; i < kR; ++i) qs[i] = p.scale * exp2_biased(127 + ex[i]);
         float o[8][4], m[kR], top[kR], l[kR];
+        uint32_t nan_seen = 0;
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
             m[i] = top[i] = kNegInf;
@@ -522,6 +548,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     vw[j] = *reinterpret_cast<const uint2*>(from + 32 * kKeyRow + (16 * u + 2 * t + (j & 1) + 8 * (j >> 1)) * kValueRow + 8 * g);
+                if (st * 32 + 32 > len_min && len_min < len_max) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vw[j] = make_uint2(without_nan(vw[j].x, nan_seen), without_nan(vw[j].y, nan_seen));
+                }
                 const uint32_t a0 = pack_f16x2(pw[2 * u][0], pw[2 * u][1]), a1 = kHalf ? 0u : pack_f16x2(pw[2 * u][2], pw[2 * u][3]);
                 const uint32_t a2 = pack_f16x2(pw[2 * u + 1][0], pw[2 * u + 1][1]),
                                a3 = kHalf ? 0u : pack_f16x2(pw[2 * u + 1][2], pw[2 * u + 1][3]);
@@ -557,7 +587,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
                 sh[warp].o[row][16 * t + 8 + d] = o[d][2 * i + 1];
             }
         }
-        __syncthreads();
+        bool nan_v = __syncthreads_or((int)nan_seen);
         constexpr int kPer = kRows * kHeadDim / (kAttWarps * 32);            // dims of one row that a thread merges: 2, 4 or 8
         const int row = (int)threadIdx.x / (kHeadDim / kPer), d0 = (int)threadIdx.x % (kHeadDim / kPer) * kPer;
         Merged<kPer> a;
@@ -571,9 +601,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
                 sh[0].top[row] = a.top;
                 sh[0].l[row] = a.l;
             }
+            if (threadIdx.x == 0) sh[0].nan_seen = nan_v;
             cluster.sync();
-            if (rank == 0)
+            if (rank == 0) {
                 a.take(C, row, d0, [&](int i) { return cluster.map_shared_rank(&sh[0], i); });
+                if (len_min < len_max)
+                    for (int i = 0; i < C; ++i) nan_v |= cluster.map_shared_rank(&sh[0], i)->nan_seen != 0;
+            }
         }
         const int at = tile * kRows + row;
         if (rank == 0 && at < rows) {
@@ -582,6 +616,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
             uint32_t* to = reinterpret_cast<uint32_t*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head + d0);
 #pragma unroll
             for (int k = 0; k < kPer; k += 2) to[k / 2] = pack_bf16x2(a.acc[k] * f, a.acc[k + 1] * f);
+            if (__builtin_expect(nan_v, 0))
+                put_nan(c, table, h, len_min & ~31, (int)min((long long)max(seq - count + tok + 1, 0), capacity),
+                        p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head, d0, kPer);
             if (p.lse && d0 == 0)
                 p.lse[(long long)(first + tok) * p.q_heads + head] = a.l == 0.f ? kNegInf : (a.m + log2f(a.l)) * 0.6931471805599453f;
         }
@@ -612,7 +649,7 @@ struct PromptShared {
     uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full[2], pv_done[2], drain;
     __align__(16) float ks[kPromptStages][4], ev[kPromptStages][4], bias[kPromptStages][4];   // per 16 keys; bias -inf: no page
     uint32_t tmem;
-    volatile int abort;
+    volatile int abort, nan_out;                       // nan_out: an output was NaN
 };
 constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + kRawStages * kRawBytes + (int)sizeof(PromptShared);
 
@@ -691,7 +728,69 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* u) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendParams p) {
+// Rows that are NaN because a V value of a key they do not see is (weight 0 times NaN): those dims once more, one row a
+// thread and without the products of the tensor cores, which takes milliseconds.  Everything is read anew, so that the
+// loop keeps nothing in registers for it; 0 in place of NaN on the way to the tiles made every
+// call 3 % slower.
+__device__ __noinline__ void rows_apart(const AttendParams& p) {
+    const Kv8Params& c = p.c;
+    const int h = blockIdx.y, r = blockIdx.z, first = c.cu ? max(c.cu[r], 0) : r;
+    const int count = c.cu ? min(c.cu[r + 1], c.tokens) - first : 1, rows = count * p.group, seq = max(c.seq_lens[r], 0);
+    const long long capacity = (long long)c.bt_cols << c.page_shift;
+    const int* table = c.block_table + r * c.bt_stride;
+    auto at = [&](int key, int& page) -> const uint8_t* {                  // K of a key, null: no page
+        page = table[key >> c.page_shift];
+        if (page < 0 || page >= c.pages) return nullptr;
+        return c.cache + (long long)page * c.page_stride + (long long)h * c.head_stride + c.k_off +
+               (long long)(key & ((1 << c.page_shift) - 1)) * c.token_stride;
+    };
+    auto value = [](uint8_t b) {
+        uint32_t lo, hi;
+        e4m3x4_to_f16(b, lo, hi);
+        return __half2float(__low2half(*reinterpret_cast<const __half2*>(&lo)));
+    };
+    for (int tile = p.tiles - 1 - (int)blockIdx.x; tile * kTileRows < rows; tile += p.tiles) {
+        const int row = tile * kTileRows + (int)threadIdx.x, tok = row / p.group, last = (min(tile * kTileRows + kTileRows, rows) - 1) / p.group;
+        if (row >= rows) break;
+        const int len = (int)min((long long)max(seq - count + tok + 1, 0), capacity);
+        const int len_max = (int)min((long long)max(seq - count + last + 1, 0), capacity);
+        const int head = h * p.group + row - tok * p.group;
+        unsigned long long dims = 0;
+#pragma unroll 1
+        for (int key = len, page; key < len_max; ++key)
+            if (const uint8_t* k = at(key, page))
+#pragma unroll 1
+                for (int d = 0; d < kHeadDim; ++d) dims |= (unsigned long long)((k[c.v_off - c.k_off + d] & 0x7f) == 0x7f) << d;
+        if (!dims) continue;
+        const uint16_t* q = p.q + (long long)(first + tok) * p.q_token + (long long)head * p.q_head;
+        float m = kNegInf;
+        double l = 0., acc[kHeadDim];
+#pragma unroll 1
+        for (int d = 0; d < kHeadDim; ++d) acc[d] = 0.;
+#pragma unroll 1
+        for (int key = 0, page; key < len; ++key) {
+            const uint8_t* k = at(key, page);
+            if (!k) continue;
+            const uint8_t* scales = c.scales + ((long long)page * c.kv_heads + h) * 2;
+            double dot = 0.;
+#pragma unroll 1
+            for (int d = 0; d < kHeadDim; ++d) dot += (double)__uint_as_float((uint32_t)q[d] << 16) * value(k[d]);
+            const float x = (float)(dot * p.scale * exp2_biased(scales[0])), m1 = fmaxf(m, x);
+            const double turn = m == m1 ? 1. : exp2((double)m - m1), w = x == kNegInf ? 0. : exp2((double)x - m1), ev = w * exp2((double)scales[1] - 127.);
+            m = m1;
+            l = l * turn + w;
+#pragma unroll 1
+            for (int d = 0; d < kHeadDim; ++d)
+                if (dims >> d & 1) acc[d] = acc[d] * turn + ev * value(k[c.v_off - c.k_off + d]);
+        }
+        uint16_t* to = p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head;
+#pragma unroll 1
+        for (int d = 0; d < kHeadDim; ++d)
+            if (dims >> d & 1) to[d] = (uint16_t)pack_bf16x2(l == 0. ? 0.f : (float)(acc[d] / l), 0.f);
+    }
+}
+
+__global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
     const Kv8Params& c = p.c;
     extern __shared__ unsigned char raw[];
     unsigned char* q_tile = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -725,7 +824,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
         mbar_init(&sh.pv_done[0], 1);
         mbar_init(&sh.pv_done[1], 1);
         mbar_init(&sh.drain, 1);
-        sh.abort = 0;
+        sh.abort = sh.nan_out = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 7) {
@@ -895,6 +994,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
                 }
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = f == 0.f ? 0.f : o[k] * f;
+                float any = o[0];
+#pragma unroll
+                for (int k = 1; k < 32; ++k) any = fmaf(o[k], 0.f, any);   // NaN if one is (or an infinity)
+                if (any != any) sh.nan_out = 1;
                 if (on) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -1025,6 +1128,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(AttendPar
     __syncthreads();
     tc_fence_after();
     if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPromptCols) : "memory");
+    if (__builtin_expect(sh.nan_out && warp < 4, 0)) rows_apart(p);
 }
 
 // ---------------------------------------------------------------- host
@@ -1123,17 +1227,23 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     p.scale = scale * 1.4426950408889634f;
     int longest = p.c.cu ? (max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens) : 1;
     if ((long long)longest * p.group > 0x7fffffffLL - 16) return kErrShape;
-    // rows a request is expected to have: the longest where the caller knows it, else the mean
-    const long long expected = (max_query_len > 0 || !p.c.cu ? (long long)longest : ((long long)tokens + p.c.batch - 1) / p.c.batch) * p.group;
+    const long long mean = ((long long)tokens + p.c.batch - 1) / p.c.batch * p.group;      // rows of a request
     // The prompt kernel's tile of 128 rows takes 1.2 us for 64 keys however few of them there are, and no tile's keys are
     // split; the other kernel's rate does not depend on either.  They meet at 740 tiles of 16 rows where the SMs are not
     // full, and at tiles of 128 rows that are 45 % full: 1 request of 128 tokens, 15/5 heads (120 tiles) 77 us against
     // 23; 8 of 32, 32/32 heads (512) 45 against 29; 16 of 256, 9/3 heads (2304) 85 against 131; 32 of 64, 32/32 heads
     // (4096, half full) 77 against 108.
-    const long long sets = (long long)p.c.kv_heads * p.c.batch, small = (expected + 15) / 16 * sets;
-    if (small >= 740 && 10 * small >= 36 * ((expected + kTileRows - 1) / kTileRows) * sets) {
-        const long long tiles = ((long long)longest * p.group + kTileRows - 1) / kTileRows;
-        p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
+    const long long sets = (long long)p.c.kv_heads * p.c.batch, small = (mean + 15) / 16 * sets;
+    // Tiles a request gets CTAs for (more are taken in turns): all that the longest can have, but CTAs with nothing to do
+    // cost 1.5 ns each, so no more than twice the mean or what fills the GPU if one request has nearly all rows.  (256
+    // requests of 4 tokens, 15/5 heads, 2048 keys, longest not known: 98 us, 457 with a CTA for every possible tile.)
+    auto tiles_of = [&](int rows) {
+        const long long tiles = ((long long)longest * p.group + rows - 1) / rows;
+        const long long likely = (mean + rows - 1) / rows * 2, some = 8192 / sets, most = likely > some ? likely : some;
+        return (int)(tiles < most ? tiles : most);
+    };
+    if (small >= 740 && 10 * small >= 36 * ((mean + kTileRows - 1) / kTileRows) * sets) {
+        p.tiles = tiles_of(kTileRows);
         const cudaError_t e = allow_shared(kv8_prompt_kernel, kPromptBytes, g_prompt_ready);
         if (e != cudaSuccess) return (int)e;
         kv8_prompt_kernel<<<dim3((unsigned)p.tiles, (unsigned)p.c.kv_heads, (unsigned)p.c.batch), kPromptThreads, kPromptBytes,
@@ -1141,8 +1251,8 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
         return (int)cudaPeekAtLastError();
     }
     const int tile_rows = (long long)longest * p.group <= 8 ? 8 : 16;
-    const long long tiles = ((long long)longest * p.group + tile_rows - 1) / tile_rows;
-    const long long items = tiles * p.c.kv_heads * p.c.batch;
+    p.tiles = tiles_of(tile_rows);
+    const long long items = (mean + tile_rows - 1) / tile_rows * sets;
     const long long steps = (((long long)p.c.bt_cols << p.c.page_shift) + 31) / 32;
     // CTAs that share the keys of one item: as many as are resident at once (two on each of 148 SMs), at least two steps
     // for each warp.  Where that leaves eight steps or more an eighth more CTAs is worth a second wave (32 requests x 5 kv
@@ -1154,7 +1264,6 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     if (fit > steps / (8 * kAttWarps)) fit = 296 / items;
     const long long share = fit < worth ? fit : worth;
     const int c = (int)(share < 1 ? 1 : (share < 8 ? share : 8));
-    p.tiles = (int)(tiles < (1 << 24) ? tiles : (1 << 24));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p.tiles * c), (unsigned)p.c.kv_heads, (unsigned)p.c.batch);
     cfg.blockDim = dim3(kAttWarps * 32);

@@ -360,6 +360,17 @@ torch::Tensor kv8_attention(const torch::Tensor& q, const torch::Tensor& cache, 
     return out;
 }
 
+std::tuple<torch::Tensor, torch::Tensor> kv8_attention_lse(const torch::Tensor& q, const torch::Tensor& cache, const torch::Tensor& scales,
+                                                           const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                                                           const std::optional<torch::Tensor>& cu_seqlens, int64_t max_query_len,
+                                                           double scale) {
+    TORCH_CHECK(q.dim() == 3, "q must be bfloat16 [tokens, heads, 64] with unit last stride");
+    torch::Tensor out = torch::empty(q.sizes(), q.options());
+    torch::Tensor lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
+    kv8_attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, out, lse);
+    return {out, lse};
+}
+
 // ---- sampling
 void sample_out(const torch::Tensor& logits, const torch::Tensor& uniform, const std::optional<torch::Tensor>& temperature,
                 double temperature_value, const std::optional<torch::Tensor>& top_k, int64_t top_k_value,
@@ -425,6 +436,9 @@ TORCH_LIBRARY_FRAGMENT(prime_kv8, m) {
     m.def("attention(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
           "int max_query_len, float scale) -> Tensor");
     m.impl("attention", torch::kCUDA, &kv8_attention);
+    m.def("attention_lse(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
+          "int max_query_len, float scale) -> (Tensor, Tensor)");
+    m.impl("attention_lse", torch::kCUDA, &kv8_attention_lse);
     m.def("attention_out(Tensor q, Tensor cache, Tensor scales, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
           "int max_query_len, float scale, Tensor(a!) out, Tensor(b!)? lse) -> ()");
     m.impl("attention_out", torch::kCUDA, &kv8_attention_out);

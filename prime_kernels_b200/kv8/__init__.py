@@ -38,6 +38,11 @@ def _attention_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max_que
     return q.new_empty(q.shape)
 
 
+@torch.library.register_fake("prime_kv8::attention_lse")
+def _attention_lse_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 @torch.library.register_fake("prime_kv8::attention_out")
 def _attention_out_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max_query_len, scale, out, lse):
     return None
@@ -45,6 +50,7 @@ def _attention_out_fake(q, cache, scales, block_table, seq_lens, cu_seqlens, max
 
 _append = torch.ops.prime_kv8.append.default
 _attention = torch.ops.prime_kv8.attention.default
+_attention_lse = torch.ops.prime_kv8.attention_lse.default
 _attention_out = torch.ops.prime_kv8.attention_out.default
 
 
@@ -78,9 +84,7 @@ def attention(q, cache, scales, block_table, seq_lens, cu_seqlens=None, *, max_q
     With ``out`` given, rows that belong to no request are left as they are there; otherwise they are undefined."""
     n, s = max_query_len or 0, HEAD_DIM ** -0.5 if scale is None else scale
     if out is None:
-        if not return_lse:
-            return _attention(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return (_attention_lse if return_lse else _attention)(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s, out, lse)
     return (out, lse) if return_lse else out

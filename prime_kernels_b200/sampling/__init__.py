@@ -11,7 +11,7 @@ and the token drawn is the lowest index at which the running sum of kept weights
 times their sum.  The most likely token always stays.  NaN and ``-inf`` are never drawn; a row of nothing else gives
 id 0 (logprob NaN).  Weights are 64-bit integers relative to the row's largest, with at least 44 fractional bits: the
 same call gives the same ids whatever else runs.  A token keeps at least one unit unless its weight underflows a
-double (below ``e**-745``), so masks of a type's lowest value are never drawn either.
+double (below ``e**-707``), so masks of a type's lowest value are never drawn either.
 """
 from __future__ import annotations
 

@@ -395,6 +395,55 @@ def test_nan_is_not_hidden(cuda_device, n, heads):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("n,group,heads,size", [(3, 2, 2, 16), (4, 5, 1, 32), (40, 3, 2, 16), (77, 4, 10, 64), (260, 3, 10, 16), (300, 7, 3, 256)])
+def test_nan_of_later_tokens(cuda_device, n, group, heads, size, planes):
+    """NaN among the V values (or in the K) of a token reaches the rows that see it, and only those."""
+    from prime_kernels_b200 import kv8
+
+    g = torch.Generator().manual_seed(n)
+    seq = [n + 201, n, n + 990]
+    table, pages = tables(g, seq, size)
+    cache, scales = pool(g, pages, heads, size, planes, cuda_device)
+    total, starts = sum(seq), np.concatenate([[0], np.cumsum(seq)])
+    k, v = torch.randn(total, heads, D, generator=g), torch.randn(total, heads, D, generator=g)
+    marks = [(0, 200, 0, 3), (0, 203, 0, 63), (1, 1, heads - 1, 17), (1, n - 1, 0, 0), (2, 990 + n // 2, heads - 1, 32),
+             (2, 990 + n // 2, heads - 1, 35)]                            # request, position, kv head, dim
+    lens, cu_all = torch.tensor(seq, dtype=torch.int32), torch.from_numpy(starts.astype(np.int32))
+    for bad in (False, True):
+        kb, vb = k.bfloat16(), v.bfloat16()
+        for r, at, h, d in marks:
+            vb[starts[r] + at, h, d] = math.nan if bad else 0.0
+        if bad:
+            kb[starts[2] + 990 + n - 1, 0, 9] = math.nan                  # the last token of all
+        kv8.append(kb.to(cuda_device), vb.to(cuda_device), cache, scales, table.to(cuda_device), lens.to(cuda_device), cu_all.to(cuda_device))
+        q = torch.randn(3 * n, group * heads, D, generator=torch.Generator().manual_seed(1)).bfloat16()
+        cu = torch.arange(0, 3 * n + 1, n, dtype=torch.int32)
+        if not bad:
+            want, want_lse, tol, tol_lse, _ = attend64(q, Held(cache, scales), table.numpy(), lens.numpy(), cu.numpy(), D ** -0.5)
+    out, lse = kv8.attention(q.to(cuda_device), cache, scales, table.to(cuda_device), lens.to(cuda_device), cu.to(cuda_device),
+                             max_query_len=n, return_lse=True)
+    out, lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    for r, at, h, d in marks:
+        sees = r * n + max(at - (seq[r] - n), 0)
+        want[sees: (r + 1) * n, h * group: (h + 1) * group, d] = math.nan
+    want[-1, :group] = want_lse[-1, :group] = math.nan
+    for got, ref, t in ((out, want, tol), (lse, want_lse, tol_lse)):
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        assert (np.abs(got - ref)[~np.isnan(ref)] <= t[~np.isnan(ref)]).all()
+
+
+@pytest.mark.parametrize("known", [False, True])
+@pytest.mark.parametrize("new", [[300] + [1] * 599, [800] + [30] * 49])
+def test_one_long_among_many(cuda_device, new, known):
+    """A request with far more rows than the mean: its tiles are taken in turns."""
+    g = torch.Generator().manual_seed(len(new))
+    cache, scales, table, lens = filled(g, [n + 20 for n in new], 10, 16, False, cuda_device)
+    q = torch.randn(sum(new), 30, D, generator=g).bfloat16()
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32)
+    run_attention(cuda_device, cache, scales, table, lens, q, cu, max_query_len=max(new) if known else None)
+
+
 def test_no_wait_gave_up(cuda_device):
     """After everything above: no bounded wait of the prompt kernel has expired."""
     from prime_kernels_b200 import _cabi
