@@ -121,6 +121,17 @@ def test_masked_and_special_logits(cuda_device, dtype, knobs):
         check(x, torch.full((len(rows),), u), knobs, cuda_device)
 
 
+@pytest.mark.parametrize("temperature", [1e-40, 1e-30, 1e-3, 0.02, 0.1, 0.4])
+@pytest.mark.parametrize("knobs", [{"top_p": 0.9}, {"top_k": 50}, {"top_k": 1000}, {"top_k": 50, "top_p": 0.7}, {"top_k": 1000, "top_p": 0.95},
+                                   {"top_k": 20000, "top_p": 0.999, "min_p": 1e-6}])
+def test_low_temperatures(cuda_device, temperature, knobs):
+    """Most of a row far below the weights that count, and border bins many times a binade wide."""
+    g = torch.Generator().manual_seed(int(1 / temperature) % 1000)
+    x = torch.randn(6, 30011, generator=g) * torch.tensor([0.2, 1.0, 3.0, 3.0, 6.0, 60.0])[:, None]
+    check(x.bfloat16().to(cuda_device), torch.rand(6, generator=g), {"temperature": temperature, **knobs}, cuda_device)
+    check(x.to(cuda_device), torch.rand(6, generator=g), {"temperature": temperature, **knobs}, cuda_device)
+
+
 def test_uniform_borders(cuda_device):
     """u = 0 draws the first kept token however small its weight, u next to 1 the last one that moves the sum."""
     from prime_kernels_b200 import sampling as S
