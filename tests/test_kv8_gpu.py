@@ -530,6 +530,61 @@ def test_refusals(cuda_device):
 
 
 # ------------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("n,heads", [(1, 5), (5, 3), (300, 10)])
+def test_graphs_and_streams(cuda_device, n, heads):
+    """Append and attention captured twice and replayed with other lengths and pages, and beside each other on two streams."""
+    from prime_kernels_b200 import kv8
+
+    dev, size = cuda_device, 16
+    g = torch.Generator().manual_seed(n + heads)
+    seq = [n + 37, n + 250, n, 0 if n == 1 else n + 3]                     # a padded batch: the last decode row has no token
+    table, pages = tables(g, [s + 100 for s in seq], size)
+    x = torch.randn(4 * n, 5 * heads, D, generator=g).bfloat16().to(dev)
+    q, k, v = x[:, : 3 * heads], x[:, 3 * heads: 4 * heads], x[:, 4 * heads:]
+    cu = None if n == 1 else torch.arange(0, 4 * n + 1, n, dtype=torch.int32, device=dev)
+    start = torch.randint(0, 127, (pages, heads, size, 2 * D), generator=g, dtype=torch.uint8)
+    lens, bt = torch.tensor(seq, dtype=torch.int32, device=dev), table.to(dev)
+
+    def held():
+        cache, scales = kv8.empty_cache(pages, heads, size, device=dev)
+        cache.view(torch.uint8).copy_(start)
+        scales.view(torch.uint8).fill_(120)
+        return cache, scales
+
+    def both(cache, scales):
+        kv8.append(k, v, cache, scales, bt, lens, cu)
+        return kv8.attention(q, cache, scales, bt, lens, cu, max_query_len=n)
+
+    def eager():
+        cache, scales = held()
+        return both(cache, scales), cache
+
+    kept = [held() for _ in range(2)]
+    both(*kept[0])
+    graphs, outs = [], []
+    for cache, scales in kept:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(both(cache, scales))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for shift in (0, 20, -9):
+        lens.copy_(torch.tensor([max(s + shift, 0) if s else 0 for s in seq], dtype=torch.int32))
+        bt.copy_(table[:, torch.arange(table.shape[1])] if shift == 0 else table.flip(0))
+        for cache, scales in kept:
+            cache.view(torch.uint8).copy_(start)
+            scales.view(torch.uint8).fill_(120)
+        want, want_cache = eager()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, (cache, _) in zip(outs, kept):
+            assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+            assert torch.equal(cache.view(torch.uint8), want_cache.view(torch.uint8))
+
+
 def test_a_decode_loop_of_all_three(cuda_device):
     """Prompt chunk, then steps of append -> attention -> logits -> sample, eager and replayed from one CUDA graph on a side
     stream: the same ids; every step checked against the definition."""
