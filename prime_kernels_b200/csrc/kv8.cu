@@ -325,6 +325,14 @@ __device__ __forceinline__ float quad_max(float v) {
     return fmaxf(v, __shfl_xor_sync(kFullMask, v, 2));
 }
 
+// 2^x / l in two factors, f and g: x is the exponent of the largest weight, -127 where all V of a row lie in pages of the
+// lowest scale, and 2^-127 alone would come out 0.  g is 1 but for those.
+__device__ __forceinline__ float unscale(float x, float l, float& g) {
+    const bool low = x < -96.f;
+    g = low ? exp2_biased(127 - 96) : 1.f;
+    return ex2(low ? x + 96.f : x) / l;
+}
+
 // 16 dims (16t .. 16t + 15) of one q row as eight f16x2 registers, divided by 2^ex so that the largest |q| of the row
 // lies in [2^7, 2^8); ex is returned.  All four lanes of the row's quad take part.
 __device__ __forceinline__ int load_q(const uint16_t* row, int t, uint32_t (&f)[8]) {
@@ -612,10 +620,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
         const int at = tile * kRows + row;
         if (rank == 0 && at < rows) {
             const int tok = at / p.group, head = h * p.group + at - tok * p.group;
-            const float f = a.l == 0.f ? 0.f : ex2(a.top - a.m) / a.l;
+            float g = 1.f;
+            const float f = a.l == 0.f ? 0.f : unscale(a.top - a.m, a.l, g);
             uint32_t* to = reinterpret_cast<uint32_t*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head + d0);
 #pragma unroll
-            for (int k = 0; k < kPer; k += 2) to[k / 2] = pack_bf16x2(a.acc[k] * f, a.acc[k + 1] * f);
+            for (int k = 0; k < kPer; k += 2) to[k / 2] = pack_bf16x2(a.acc[k] * f * g, a.acc[k + 1] * f * g);
             if (__builtin_expect(nan_v, 0))
                 put_nan(c, table, h, len_min & ~31, (int)min((long long)max(seq - count + tok + 1, 0), capacity),
                         p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head, d0, kPer);
@@ -974,11 +983,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[at & 1]);                           // two: a warp may be a step ahead of another
             }
-            float f = 0.f;
+            float f = 0.f, g = 1.f;
             if (steps > 0) {
                 warp_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1);
                 tc_fence_after();
-                f = l == 0.f ? 0.f : ex2(top - m) / l;
+                f = unscale(top - m, l, g);
             }
             int again = tid;                                               // worked out once more: not kept in registers over the loop
             asm volatile("" : "+r"(again));
@@ -993,7 +1002,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = f == 0.f ? 0.f : o[k] * f;
+                for (int k = 0; k < 32; ++k) o[k] = l == 0.f ? 0.f : o[k] * f * g;  // l = 0: sees no key
                 float any = o[0];
 #pragma unroll
                 for (int k = 1; k < 32; ++k) any = fmaf(o[k], 0.f, any);   // NaN if one is (or an infinity)
