@@ -1166,7 +1166,8 @@ int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     if (a->batch == 0 || tokens == 0) return -1;                             // nothing to do
     if (!a->cache || !a->scales || !a->seq_lens || (a->bt_cols > 0 && !a->block_table)) return kErrNull;
     if (reinterpret_cast<uintptr_t>(a->cache) % 16 || reinterpret_cast<uintptr_t>(a->scales) % 2 || a->k_off % 16 || a->v_off % 16 || a->page_stride % 16 ||
-        a->token_stride % 16 || a->head_stride % 16)
+        a->token_stride % 16 || a->head_stride % 16 || reinterpret_cast<uintptr_t>(a->block_table) % 4 ||
+        reinterpret_cast<uintptr_t>(a->seq_lens) % 4 || reinterpret_cast<uintptr_t>(a->cu_seqlens) % 4)
         return kErrAlign;
     if (!a->cu_seqlens && tokens < a->batch) return kErrShape;
     c.cache = static_cast<uint8_t*>(a->cache);

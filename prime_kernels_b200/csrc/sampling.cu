@@ -908,6 +908,8 @@ extern "C" int pk_sample(const PkSampleArgs* a) {
     if (!a->logits || !a->uniform || !a->ids) return kErrNull;
     const int es = a->dtype == 2 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(a->logits) % es || reinterpret_cast<uintptr_t>(a->ids) % 8) return kErrAlign;
+    for (const void* x : {a->uniform, a->temperature, a->top_k, a->top_p, a->min_p, static_cast<const void*>(a->logprobs)})
+        if (reinterpret_cast<uintptr_t>(x) % 4) return kErrAlign;
     // CTAs per row: as many as there are SMs for while rows are few (two or four for 64 rows make no difference: 31.6 us
     // and 31.1 with top-p), and enough for a slice of 64 KB, two of which fit an SM beside the 48 KB of tables.
     int cluster = 1;
