@@ -189,7 +189,8 @@ int pk_decode_wait_probe(void* workspace, size_t bytes, unsigned rounds, void* s
  * for V (x = value * 2^(scale - 127)); head_dim is 64.  K and V of (page, head, slot) are 64 bytes at
  * page * page_stride + head * head_stride + slot * token_stride + k_off / v_off; all strides and offsets are bytes and
  * multiples of 16, page_size is 16, 32, 64, 128 or 256.  block_table int32 [batch][bt_cols] (row stride bt_stride
- * elements); an entry outside 0..pages-1 stands for no page: nothing is stored there and its tokens are masked.
+ * elements, bt_cols * page_size at most 2^31 - 2^16); an entry outside 0..pages-1 stands for no page: nothing is stored
+ * there and its tokens are masked.
  * seq_lens int32 [batch] include the new tokens.  cu_seqlens int32 [batch + 1]: request r owns rows
  * cu[r]..cu[r+1]-1 of q / k / v, the last cu[r+1]-cu[r] positions of its sequence; NULL: row r is request r. */
 typedef struct PkKv8Cache {

@@ -1162,7 +1162,8 @@ int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     int shift = 4;
     while (shift < 8 && (1 << shift) != a->page_size) ++shift;
     if ((1 << shift) != a->page_size) return kErrBlock;                      // 16, 32, 64, 128 or 256
-    if ((long long)a->bt_cols * a->page_size > 0x7fffffffLL) return kErrMaxSeq;
+    // the kernels look up pages up to 32 steps of 64 keys past a row's last key, in 32 bits
+    if ((long long)a->bt_cols * a->page_size > 0x7fff0000LL) return kErrMaxSeq;
     if (a->batch == 0 || tokens == 0) return -1;                             // nothing to do
     if (!a->cache || !a->scales || !a->seq_lens || (a->bt_cols > 0 && !a->block_table)) return kErrNull;
     if (reinterpret_cast<uintptr_t>(a->cache) % 16 || reinterpret_cast<uintptr_t>(a->scales) % 2 || a->k_off % 16 || a->v_off % 16 || a->page_stride % 16 ||
@@ -1236,7 +1237,7 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     p.group = q_heads / p.c.kv_heads;
     p.scale = scale * 1.4426950408889634f;
     int longest = p.c.cu ? (max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens) : 1;
-    if ((long long)longest * p.group > 0x7fffffffLL - 16) return kErrShape;
+    if ((long long)(p.c.cu ? tokens : 1) * p.group > 0x3fffff00LL) return kErrShape;     // row + a turn of tiles: 32 bits
     const long long mean = ((long long)tokens + p.c.batch - 1) / p.c.batch * p.group;      // rows of a request
     // The prompt kernel's tile of 128 rows takes 1.2 us for 64 keys however few of them there are, and no tile's keys are
     // split; the other kernel's rate does not depend on either.  They meet at 740 tiles of 16 rows where the SMs are not
