@@ -10,6 +10,7 @@
 #include <torch/all.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <tuple>
 
 #include "../../include/prime_kernels_b200.h"
@@ -407,7 +408,7 @@ void sample_out(const torch::Tensor& logits, const torch::Tensor& uniform, const
     a.top_p = opt_ptr(top_p);
     a.min_p = opt_ptr(min_p);
     a.temperature_value = (float)temperature_value;
-    a.top_k_value = (int)std::min<int64_t>(top_k_value, INT32_MAX);
+    a.top_k_value = (int)std::clamp<int64_t>(top_k_value, 0, INT32_MAX);
     a.top_p_value = (float)top_p_value;
     a.min_p_value = (float)min_p_value;
     a.ids = ids.data_ptr();
