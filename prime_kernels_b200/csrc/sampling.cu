@@ -146,6 +146,21 @@ __device__ __forceinline__ unsigned long long token_of(uint32_t key, int index) 
     return ((unsigned long long)key << 32) | (uint32_t)~index;
 }
 
+// floor(part * whole) for 0 <= part < 1, exactly (a double holds 53 of the 62 bits of a sum of weights: among equal tokens the
+// product would fall beside the running sum that it is equal to); `exact`: nothing was cut off
+__device__ __forceinline__ unsigned long long part_of(float part, unsigned long long whole, bool& exact) {
+    const uint32_t b = __float_as_uint(part), e = max(b >> 23, 1u), m = (b & 0x7fffffu) | (b >> 23 ? 0x800000u : 0u);
+    const int shift = 150 - (int)e;                           // part = m * 2^-shift, shift 24..149
+    const unsigned long long lo = m * whole, hi = __umul64hi(m, whole);
+    if (shift < 64) {
+        exact = (lo & ((1ull << shift) - 1)) == 0;
+        return (hi << (64 - shift)) | (lo >> shift);
+    }
+    const int s = min(shift - 64, 63);                        // hi < 2^23
+    exact = lo == 0 && (hi & ((1ull << s) - 1)) == 0;
+    return hi >> s;
+}
+
 // double(v) by integer operations (a conversion costs as much as four 64-bit products); subnormals come out wrong by
 // less than 2^-126 and infinity as 2^128
 __device__ __forceinline__ double widen(float v) {
@@ -551,13 +566,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleParams 
     const int top_k = p.top_k ? p.top_k[row] : p.top_k_v;
     const float given_p = p.top_p ? p.top_p[row] : p.top_p_v, top_p = fmaxf(given_p, 0.f);
     const float min_p = p.min_p ? p.min_p[row] : p.min_p_v;
-    const double u = (double)fmaxf(p.uniform[row], 0.f);                     // NaN: 0
+    const float u = fmaxf(p.uniform[row], 0.f);                              // NaN: 0
     const bool by_k = top_k > 0 && top_k < p.vocab, by_p = given_p < 1.f;                   // NaN: off
-    auto least_target = [](double part, unsigned long long whole) {          // smallest integer >= part * whole, 1..whole
-        const double t = ceil(part * (double)whole);
-        return t < 1.0 ? 1ull : min((unsigned long long)t, whole);
+    auto least_target = [](float part, unsigned long long whole) {           // smallest integer >= part * whole, 1..whole; part < 1
+        bool exact;
+        const unsigned long long t = part_of(part, whole, exact);
+        return max(t + (exact ? 0 : 1), 1ull);
     };
-    auto draw_target = [&](unsigned long long whole) { return u >= 1.0 ? whole - 1 : min((unsigned long long)(u * (double)whole), whole - 1); };
+    auto draw_target = [&](unsigned long long whole) {
+        bool exact;
+        return u >= 1.f ? whole - 1 : part_of(u, whole, exact);
+    };
     const unsigned long long least_w = weight.least(min_p);
 
     // index order: warp w of the CTA owns a contiguous run of the slice
