@@ -214,9 +214,12 @@ int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long long q_token_s
                      long long out_token_stride, long long out_head_stride, void* lse, int tokens, int q_heads,
                      int max_query_len, float scale, void* stream);
 
-/* Bounded barrier waits of the kernel for many query tokens that expired since load (0 = healthy; -1 = CUDA error).
- * Synchronises. */
+/* Bounded barrier waits of the kernel for many query tokens that expired on the current device since load (0 = healthy; -1 =
+ * CUDA error).  Rows that such a launch could not finish are NaN, out and lse.  Waits for all work on the device.
+ * pk_kv8_set_wait_limit: bound, in polls, of every such wait of later launches (0: a wait that is not over at once has
+ * expired; negative: the default, 2^20). */
 long long pk_kv8_wait_timeouts(void);
+void pk_kv8_set_wait_limit(int polls);
 
 /* ---------------------------------------------------------------- sampling */
 

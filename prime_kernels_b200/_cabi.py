@@ -85,6 +85,7 @@ SYMBOLS = {
     "pk_kv8_append": (ci, [ctypes.POINTER(PkKv8Cache), vp, ll, ll, vp, ll, ll, ci, vp]),
     "pk_kv8_attention": (ci, [ctypes.POINTER(PkKv8Cache), vp, ll, ll, vp, ll, ll, vp, ci, ci, ci, cf, vp]),
     "pk_kv8_wait_timeouts": (ll, []),
+    "pk_kv8_set_wait_limit": (None, [ci]),
     "pk_sample": (ci, [ctypes.POINTER(PkSampleArgs)]),
     "mk_query": (ci, [ip] * 7),
     "mk_workspace_bytes": (sz, [ci, ci]),

@@ -234,6 +234,7 @@ struct AttendParams {
     long long o_token, o_head;
     float* lse;                                        // [tokens, q heads] or null
     int q_heads, group, tiles;
+    unsigned wait_limit;                               // polls of a wait of the prompt kernel
     float scale;                                       // softmax scale * log2(e)
 };
 
@@ -653,6 +654,7 @@ constexpr int kRawStages = 3, kRawBytes = kTileKeys * 128;              // e4m3 
 constexpr int kPromptThreads = 256, kProducers = 128;
 constexpr uint32_t kPromptCols = 256, kColP = 128, kColO = 192;            // S in columns 0..127, P in 128..191, two of each
 constexpr float kLazy = 8.f;
+constexpr unsigned kWaitLimit = 1u << 20;
 
 struct PromptShared {
     uint64_t full[kPromptStages], empty[kPromptStages], q_full, s_full[2], p_full[2], pv_done[2], drain;
@@ -660,28 +662,39 @@ struct PromptShared {
     uint32_t tmem;
     volatile int abort, nan_out;                       // nan_out: an output was NaN
 };
-constexpr int kPromptBytes = 1024 + kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + kRawStages * kRawBytes + (int)sizeof(PromptShared);
+constexpr int kPromptBytes = kTileRows * 128 + kPromptStages * 2 * kTileKeys * 128 + kRawStages * kRawBytes + (int)sizeof(PromptShared);
 
 __device__ unsigned int g_kv8_wait_timeouts;
 
-// Bounded wait: gives up after some seconds, or as soon as another thread of the CTA has.
-__device__ __forceinline__ void prompt_poll(PromptShared& sh, uint64_t* bar, uint32_t parity) {
-    for (uint32_t n = 0; n < (1u << 20); ++n) {
-        if (mbar_test(bar, parity & 1u)) return;
-        if ((n & 63) == 63 && sh.abort) return;
-    }
+// Bounded waits: false once `limit` polls are over, or as soon as another thread of the CTA has given up.
+// Whoever gets false touches nothing that the wait guards and leaves its loop: the parts that depend on it run out in turn,
+// the softmax warps agree on it at the end of the tile, and their rows become NaN.
+__device__ __forceinline__ void gave_up(PromptShared& sh) {
     if (!sh.abort) {
         sh.abort = 1;
         atomicAdd(&g_kv8_wait_timeouts, 1u);
     }
 }
-__device__ __forceinline__ void prompt_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
-    if (__builtin_expect(!mbar_test(bar, parity & 1u), 0)) prompt_poll(sh, bar, parity);
+__device__ __forceinline__ bool prompt_poll(PromptShared& sh, uint64_t* bar, uint32_t parity, unsigned limit) {
+    for (uint32_t n = 0; n < limit; ++n) {
+        if (mbar_test(bar, parity & 1u)) return true;
+        if ((n & 63) == 63 && sh.abort) return false;
+    }
+    gave_up(sh);
+    return false;
+}
+__device__ __forceinline__ bool prompt_wait(PromptShared& sh, uint64_t* bar, uint32_t parity, unsigned limit) {
+    return __builtin_expect(mbar_test(bar, parity & 1u), 1) || prompt_poll(sh, bar, parity, limit);
 }
 // The same for a whole warp whose next instruction is a warp-wide one: lanes may leave the polling loop apart.
-__device__ __forceinline__ void warp_wait(PromptShared& sh, uint64_t* bar, uint32_t parity) {
-    prompt_wait(sh, bar, parity);
-    __syncwarp();
+__device__ __forceinline__ bool warp_wait(PromptShared& sh, uint64_t* bar, uint32_t parity, unsigned limit) {
+    return __all_sync(kFullMask, prompt_wait(sh, bar, parity, limit));
+}
+__device__ __forceinline__ bool any_of_softmax(bool mine) {                 // of the 128 threads of warps 0-3
+    uint32_t r;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(r) : "r"((uint32_t)mine) : "memory");
+    return r != 0;
 }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -799,10 +812,24 @@ __device__ __noinline__ void rows_apart(const AttendParams& p) {
     }
 }
 
+// The CTA gave up a wait in this tile: its rows, and those of the tiles it would have taken after it.
+__device__ __noinline__ void rows_given_up(const AttendParams& p, int tile) {
+    const Kv8Params& c = p.c;
+    const int h = blockIdx.y, r = blockIdx.z, first = c.cu ? max(c.cu[r], 0) : r;
+    const int rows = (c.cu ? min(c.cu[r + 1], c.tokens) - first : 1) * p.group;
+    for (; tile * kTileRows < rows; tile += p.tiles) {
+        const int row = tile * kTileRows + (int)threadIdx.x, tok = row / p.group, head = h * p.group + row - tok * p.group;
+        if (row >= rows) break;
+        uint4* to = reinterpret_cast<uint4*>(p.out + (long long)(first + tok) * p.o_token + (long long)head * p.o_head);
+        for (int i = 0; i < 8; ++i) to[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+        if (p.lse) p.lse[(long long)(first + tok) * p.q_heads + head] = __int_as_float(0x7fffffff);
+    }
+}
+
 __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __grid_constant__ AttendParams p) {
     const Kv8Params& c = p.c;
-    extern __shared__ unsigned char raw[];
-    unsigned char* q_tile = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    // aligned by its declaration: addresses known when it is compiled take no registers (260 us with a base rounded up)
+    extern __shared__ __align__(1024) unsigned char q_tile[];
     unsigned char* kv_tiles = q_tile + kTileRows * 128;                    // per stage: K, V
     unsigned char* raw_ring = kv_tiles + kPromptStages * 2 * kTileKeys * 128;
     PromptShared& sh = *reinterpret_cast<PromptShared*>(raw_ring + kRawStages * kRawBytes);
@@ -886,9 +913,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
             }
             const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
             float m = kNegInf, top = kNegInf, l = 0.f;
-            for (int i = 0; i < steps; ++i) {
+            int i = 0;                                                     // short of `steps` where a wait gave up
+            for (; i < steps; ++i) {
                 const uint32_t at = n + i, stage = at % kPromptStages;
-                warp_wait(sh, &sh.s_full[at & 1], at >> 1);
+                if (!warp_wait(sh, &sh.s_full[at & 1], at >> 1, p.wait_limit)) break;
                 tc_fence_after();
                 float s[kTileKeys];
                 tmem_ld32(lanes + (at & 1) * kTileKeys, s);
@@ -958,7 +986,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                     use(k);
                 }
                 if (i > 1) {                                               // this P has been read
-                    warp_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1);
+                    if (!warp_wait(sh, &sh.pv_done[at & 1], (at - 2) >> 1, p.wait_limit)) break;
                     tc_fence_after();
                 }
                 tmem_st16(lanes + kColP + (at & 1) * 32, pk);
@@ -968,7 +996,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
 #pragma unroll
                 for (int u = 0; u < 4; ++u) l += sum[u].x + sum[u].y;
                 if (__builtin_expect(i > 0 && __any_sync(kFullMask, turn != 1.f), 0)) {
-                    warp_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1);
+                    if (!warp_wait(sh, &sh.pv_done[(at - 1) & 1], (at - 1) >> 1, p.wait_limit)) break;
                     tc_fence_after();
 #pragma unroll
                     for (int d = 0; d < 2; ++d) {
@@ -983,9 +1011,14 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[at & 1]);                           // two: a warp may be a step ahead of another
             }
+            if (any_of_softmax(i < steps || (steps > 0 && !warp_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1, p.wait_limit)))) {
+                tmem_st_wait();                                            // on its way when the loop was left
+                tc_fence_before();
+                rows_given_up(p, tile);
+                break;
+            }
             float f = 0.f, g = 1.f;
             if (steps > 0) {
-                warp_wait(sh, &sh.pv_done[(n + steps - 1) & 1], (n + steps - 1) >> 1);
                 tc_fence_after();
                 f = unscale(top - m, l, g);
             }
@@ -1051,11 +1084,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                 cp_async16(to + 3 * kProducers * 16, src1 + v_from_k, on1);
                 cp_async_commit();
             };
-            auto produce = [&](int i) {
+            auto produce = [&](int i) -> bool {
                 const uint32_t at = n + i, stage = at % kPromptStages;
                 fetch(i + kRawStages - 1);                                 // steps past the last fetch zeros
                 cp_async_wait<kRawStages - 1>();
-                if (at >= kPromptStages) warp_wait(sh, &sh.empty[stage], at / kPromptStages - 1);
+                if (at >= kPromptStages && !warp_wait(sh, &sh.empty[stage], at / kPromptStages - 1, p.wait_limit)) return false;
                 unsigned char* k_tile = kv_tiles + stage * 2 * kTileKeys * 128;
                 const unsigned char* raw16 = mine + (i % kRawStages) * kRawBytes;
 #pragma unroll
@@ -1080,15 +1113,17 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.full[stage]);
+                return true;
             };
             for (int i = 0; i < kRawStages - 1; ++i) fetch(i);
+            bool fed = true, ok = true;                                    // no wait of the warp for a stage, of this lane for products, gave up
             if (warp < 7) {
-                for (int i = 0; i < steps; ++i) produce(i);
+                for (int i = 0; fed && i < steps; ++i) fed = produce(i);
             } else {
                 const uint64_t dq = tile_desc(q_tile);
-                auto scores = [&](int i) {
+                auto scores = [&](int i) -> bool {
                     const uint32_t at = n + i, stage = at % kPromptStages;
-                    prompt_wait(sh, &sh.full[stage], at / kPromptStages);
+                    if (!prompt_wait(sh, &sh.full[stage], at / kPromptStages, p.wait_limit)) return false;
                     tc_fence_after();
                     const uint64_t dk = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128);
 #pragma unroll
@@ -1096,40 +1131,43 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
                         mma_ss(tmem + (at & 1) * kTileKeys, dq + 2 * k, dk + 2 * k, kIdescQK, k > 0);
                     mma_commit(&sh.s_full[at & 1]);
                     mbar_arrive(&sh.s_full[at & 1]);                       // hands on the scales that came with the tile
+                    return true;
                 };
                 // two tiles ahead of the products: a tile's stage is free once the products of four steps before are done
-                for (int i = 0; i < min(2, steps); ++i) produce(i);
-                if (lane == 0) {
-                    prompt_wait(sh, &sh.q_full, tiles_done);
-                    if (steps > 0) scores(0);
-                }
+                for (int i = 0; fed && i < min(2, steps); ++i) fed = produce(i);
+                if (lane == 0) ok = prompt_wait(sh, &sh.q_full, tiles_done, p.wait_limit) && (steps == 0 || scores(0));
                 __syncwarp();
                 for (int i = 0; i < steps; ++i) {
-                    if (lane == 0 && i + 1 < steps) scores(i + 1);
+                    if (lane == 0 && ok && i + 1 < steps) ok = scores(i + 1);
                     __syncwarp();
-                    if (i + 2 < steps) produce(i + 2);
-                    if (lane == 0) {
+                    if (fed && i + 2 < steps) fed = produce(i + 2);
+                    if (lane == 0 && ok) {
                         const uint32_t at = n + i, stage = at % kPromptStages;
-                        prompt_wait(sh, &sh.p_full[at & 1], at >> 1);
-                        tc_fence_after();
-                        const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
+                        ok = prompt_wait(sh, &sh.p_full[at & 1], at >> 1, p.wait_limit);
+                        if (ok) {
+                            tc_fence_after();
+                            const uint64_t dv = tile_desc(kv_tiles + stage * 2 * kTileKeys * 128 + kTileKeys * 128);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)                        // 16 keys = 2048 bytes of V, 8 columns of P
-                            mma_ts(tmem + kColO, tmem + kColP + (at & 1) * 32 + 8 * k, dv + 128 * k, kIdescPV, i > 0 || k > 0);
-                        mma_commit(&sh.empty[stage]);
-                        mma_commit(&sh.pv_done[at & 1]);
+                            for (int k = 0; k < 4; ++k)                    // 16 keys = 2048 bytes of V, 8 columns of P
+                                mma_ts(tmem + kColO, tmem + kColP + (at & 1) * 32 + 8 * k, dv + 128 * k, kIdescPV, i > 0 || k > 0);
+                            mma_commit(&sh.empty[stage]);
+                            mma_commit(&sh.pv_done[at & 1]);
+                        }
                     }
                     __syncwarp();
                 }
             }
             cp_async_wait<0>();                                            // the next tile's copies go to the same places
+            if (!__all_sync(kFullMask, fed && ok)) break;
         }
         n += (uint32_t)steps;
     }
     if (warp == 7) {
         if (lane == 0) {                                                   // nothing is in flight when the memory goes
-            mma_commit(&sh.drain);
-            prompt_wait(sh, &sh.drain, 0);
+            mma_commit(&sh.drain);                                         // also after a wait that gave up: whoever did
+            unsigned polls = 0;
+            while (!mbar_test(&sh.drain, 0) && ++polls < kWaitLimit) {}
+            if (polls == kWaitLimit) gave_up(sh);
         }
         __syncwarp();
     }
@@ -1137,7 +1175,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2) kv8_prompt_kernel(const __g
     __syncthreads();
     tc_fence_after();
     if (warp == 7) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPromptCols) : "memory");
-    if (__builtin_expect(sh.nan_out && warp < 4, 0)) rows_apart(p);
+    if (__builtin_expect(sh.nan_out && warp < 4, 0) && !sh.abort) rows_apart(p);
 }
 
 // ---------------------------------------------------------------- host
@@ -1153,6 +1191,7 @@ template <typename K> cudaError_t allow_shared(K kernel, int bytes, std::atomic<
     return e;
 }
 std::atomic<unsigned long long> g_prompt_ready{0}, g_attend_ready[2];
+std::atomic<unsigned> g_wait_limit{kWaitLimit};
 
 int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
     if (!a) return kErrNull;
@@ -1186,12 +1225,18 @@ int kv8_params(const PkKv8Cache* a, int tokens, Kv8Params& c) {
 
 }  // namespace pk
 
-// Bounded waits of the prompt kernel that gave up since the library was loaded (0 in normal operation; a launch that
-// counted one produced invalid output).  Synchronises the device.
+// Bounded waits of the prompt kernel that gave up on the current device since the library was loaded (0 in normal
+// operation; rows of a launch that could not be finished are NaN).  Waits for all work on the device.
 extern "C" long long pk_kv8_wait_timeouts(void) {
     unsigned int n = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;
     if (cudaMemcpyFromSymbol(&n, pk::g_kv8_wait_timeouts, sizeof(n)) != cudaSuccess) return -1;
     return (long long)n;
+}
+
+// Polls after which a wait of later launches gives up; 0: at the first one that is not over already; < 0: the default.
+extern "C" void pk_kv8_set_wait_limit(int polls) {
+    pk::g_wait_limit.store(polls < 0 ? pk::kWaitLimit : (unsigned)polls, std::memory_order_relaxed);
 }
 
 extern "C" int pk_kv8_append(const PkKv8Cache* cache, const void* k, long long k_token_stride, long long k_head_stride,
@@ -1255,6 +1300,7 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     };
     if (small >= 740 && 10 * small >= 36 * ((mean + kTileRows - 1) / kTileRows) * sets) {
         p.tiles = tiles_of(kTileRows);
+        p.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
         const cudaError_t e = allow_shared(kv8_prompt_kernel, kPromptBytes, g_prompt_ready);
         if (e != cudaSuccess) return (int)e;
         kv8_prompt_kernel<<<dim3((unsigned)p.tiles, (unsigned)p.c.kv_heads, (unsigned)p.c.batch), kPromptThreads, kPromptBytes,

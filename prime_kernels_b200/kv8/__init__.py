@@ -18,12 +18,12 @@ from __future__ import annotations
 
 import torch
 
-from .._cabi import load_ops
+from .._cabi import library, load_ops
 from ..geometry import HEAD_DIM
 
 load_ops()
 
-__all__ = ["PAGE_SIZES", "empty_cache", "append", "attention", "dequantise"]
+__all__ = ["PAGE_SIZES", "empty_cache", "append", "attention", "check_status", "dequantise"]
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -88,6 +88,21 @@ def attention(q, cache, scales, block_table, seq_lens, cu_seqlens=None, *, max_q
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _attention_out(q, cache, scales, block_table, seq_lens, cu_seqlens, n, s, out, lse)
     return (out, lse) if return_lse else out
+
+
+_expired: dict[int, int] = {}
+
+
+def check_status(device="cuda") -> None:
+    """Synchronise and raise if a bounded device-side wait of an earlier :func:`attention` call on ``device`` gave up (the
+    rows that such a call could not finish are NaN, out and lse)."""
+    with torch.cuda.device(device):
+        at, n = torch.cuda.current_device(), library().pk_kv8_wait_timeouts()
+    if n < 0:
+        raise RuntimeError("kv8: the device could not be asked for expired waits")
+    new, _expired[at] = n - _expired.get(at, 0), n
+    if new:
+        raise RuntimeError(f"kv8 attention failed on the device: {new} bounded waits gave up")
 
 
 def dequantise(cache, scales):

@@ -19,3 +19,16 @@ def cuda_device():
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def kv8_waits_hold(request):
+    """After each test of the 8-bit cache: no bounded wait of its attention kernels has expired in it."""
+    yield
+    if request.module.__name__.startswith("test_kv8"):
+        import torch
+
+        if torch.cuda.is_available():
+            from prime_kernels_b200 import kv8
+
+            kv8.check_status()
