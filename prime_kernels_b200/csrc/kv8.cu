@@ -214,8 +214,13 @@ __global__ void __launch_bounds__(256, kGroup == 1 ? 2 : 3) kv8_append_kernel(Ap
 // are interleaved by byte permutation.
 //
 // V scales differ from page to page, so weights enter the second product as 2^(s + eV - top) with a running maximum
-// `top` of s + eV of their own, apart from the running maximum of s that the sum uses: neither over- nor underflows
-// whatever the scales are, as long as 2^(s - m) does not.
+// `top` of s + eV of their own, apart from the running maximum of s that the sum uses: a page's scale can neither overflow
+// them nor push all of them below f16.  What they lose: a weight is off by 2^-11 of itself or by 2^-25 of the row's largest
+// product of weight and V scale, whichever is more, which is below the rounding of a bf16 output unless the heavier tokens
+// hold next to nothing in a dim.  So with equal scores a page keeps its full precision in every dim down to a V scale
+// of 2^-13 of the largest, loses bits below that, and from 2^-25 on adds nothing.  (bf16 would reach further with 2^-9 of
+// each weight; weights apart from scales would take an accumulator for each page.)  Sums and maxima are fp32, exponentials
+// ex2.approx (2^-22).
 //
 // A key that only later tokens of a tile see has weight 0 for the others, and 0 * NaN is NaN: where rows of a tile differ
 // in what they see, NaN among the V values is taken for 0 in the product and put into the rows that see it at the end

@@ -80,6 +80,9 @@ def attention(q, cache, scales, block_table, seq_lens, cu_seqlens=None, *, max_q
     Token ``j`` of a request with ``n`` rows sees its first ``seq_len - n + j + 1`` positions; query head ``a`` reads kv
     head ``a // (q_heads // kv_heads)``.  A row that sees no key gets 0 (lse ``-inf``).  ``max_query_len``: the longest
     request's rows, where the caller knows it (every row is computed whatever it says); ``scale`` defaults to 1/8.
+    Weights and V values meet in f16: a weight is off by ``2**-11`` of itself or ``2**-25`` of the row's largest product of
+    weight and V scale, so what pages of a V scale below ``2**-13`` of another's add to dims in which that one holds nothing
+    loses bits, and is lost from ``2**-25`` on.
     Returns bf16 ``out`` of q's shape, or ``(out, lse)`` with the natural-log normaliser fp32 ``[tokens, q_heads]``.
     With ``out`` given, rows that belong to no request are left as they are there; otherwise they are undefined."""
     n, s = max_query_len or 0, HEAD_DIM ** -0.5 if scale is None else scale
