@@ -75,8 +75,10 @@ __device__ __forceinline__ bool request_of(const Kv8Params& p, int t, int& r, in
 // One warp per (16 consecutive rows, kv head), or per (request, kv head) with one token each.  Among its rows the warp
 // looks for the first new token of a page, which leads: it stores all new tokens of that page, K and V, whether or not
 // they lie among the warp's rows.  16 of them are kept in registers between the maximum and the values; more (pages of 32
-// slots and up) are read again, from L2.  Bound by bytes: 17.4 k tokens x 32 heads out of fused projection rows, 214 MB, in
-// 43 us (0.76 of the measured copy bandwidth); a warp per row, all but the leaders of which left at once, took 134 us.
+// slots and up) are read again, from L2.  17.4 k tokens x 32 heads out of fused projection rows, 214 MB, take 43 us on the
+// device (0.76 of the measured copy bandwidth; 42 us with pages of 16 slots, 56 and 64 us with 128 and 256): bytes, and what
+// a warp leaves unused of them, as it loads a page only when the one before is stored.  A warp per row, all but the leaders
+// of which left at once, took 134 us.
 struct AppendParams {
     Kv8Params c;
     const uint16_t *k, *v;
@@ -226,9 +228,10 @@ __global__ void __launch_bounds__(256, kGroup == 1 ? 2 : 3) kv8_append_kernel(Ap
 // in what they see, NaN among the V values is taken for 0 in the product and put into the rows that see it at the end
 // (the prompt kernel computes rows that it spoiled once more).
 //
-// Bound by the bytes of the cache where there are many, by the chain of dependent reads at the start (length, page, page's
-// data) and the merge where there are few.  64 requests of up to 8192 tokens, 15/5 heads: 44 us, 4.8 TB/s, 0.73 of the
-// measured copy bandwidth.  Steps of 16 keys read ahead in registers took 60 us (295 instructions a step, two thirds of
+// Bound by the bytes of the cache where there are many and lengths are alike, by the longest item where they differ (the
+// split is one number for a launch), by the chain of dependent reads at the start (length, page, page's data) and the
+// merge where there are few.  64 requests of 2144 to 8192 tokens, 15/5 heads: 45 us on the device, 4.7 TB/s, 0.72 of the
+// measured copy bandwidth; one CTA an item, the longest of which has 1.47 times the mean place's keys.  Steps of 16 keys read ahead in registers took 60 us (295 instructions a step, two thirds of
 // them not products), with a ring 52 us; 32 keys share the page lookups, maxima and rescaling (only where a maximum
 // moved).
 struct AttendParams {
@@ -647,11 +650,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, 16 / kAttWarps) kv8_attend_ker
 // memory.  One CTA holds one tile; warps 0-3 own a row a thread (softmax), warps 4-7 turn e4m3 pages into swizzled f16
 // tiles of 64 keys, and a thread of warp 7 issues the products: eight warps, two on each scheduler, 128 registers a thread.
 // (Two warps with all of the pages made the softmax warps beside them the slowest; sparing warp 7 its share made the other
-// three so: 259, 263 and 269 us where this takes 252.)  S is double-buffered, so the next scores are computed
+// three so: 259, 263 and 269 us where this took 252.)  S is double-buffered, so the next scores are computed
 // while the softmax works, and two CTAs share an SM (256 columns of tensor memory each), so one's products run under
 // the other's exponentials.
 //
-// Bound by the exponentials: 16 a clock and SM against 64 x 4 flops each, a quarter of the tensor peak at head dim 64.
+// The exponentials are the floor (16 a clock and SM against 64 x 4 flops each, a quarter of the tensor peak at head dim 64:
+// 81 us for four chunks of up to 2048 tokens behind up to 6144, 15/5 heads).  Bound by the chain of a step, scores ->
+// maximum -> exponentials -> weights, with two CTAs on an SM to hide it: 246 us on the device there, 2750 clocks a step at
+// 1965 MHz for the place with most of them (176, the mean is 153); no unit is busy.  96 bytes of registers are spilled.
 // `top` is raised only where a row's maximum has grown by 2^8, so that the accumulator is rarely rescaled; f16 holds 2^8
 // times the weights.
 constexpr int kTileRows = 128, kTileKeys = 64, kPromptStages = 4;
@@ -1320,7 +1326,8 @@ extern "C" int pk_kv8_attention(const PkKv8Cache* cache, const void* q, long lon
     // for each warp.  Where that leaves eight steps or more an eighth more CTAs is worth a second wave (32 requests x 5 kv
     // heads at 8192 keys: 27.7 us with two CTAs an item, 38.9 with one); with two steps it is not (16 requests at 2048
     // keys: 13.1 us with four, 10.0 with three).  Fewer than two steps cost more in merging than they save (8 requests of
-    // 5 tokens at 2047 keys: 12.3 us, 9.4).
+    // 5 tokens at 2047 keys: 12.3 us, 9.4).  Lengths are on the device, so the table's width stands for them: the same 8
+    // requests with a table for 8192 keys take 12.4 us, one request of 520 keys 6.1 us with either.
     const long long worth = steps / (2 * kAttWarps);
     long long fit = 340 / items;
     if (fit > steps / (8 * kAttWarps)) fit = 296 / items;
